@@ -482,6 +482,68 @@ int sc_attention_combine(const float* part_out, const float* part_lse,
                          int rows, int nparts, int D, sc_bf16* out,
                          float* lse_out, void* stream);
 
+/* --------------------------------------------------------------------------
+ * Group decode: several sequences (samples or beams) over one prompt.
+ * ------------------------------------------------------------------------ */
+
+/* q/k RMS norm, rotary positions with several axes and the KV append, one launch.
+ *
+ * Replaces what mlx-vlm's `_prepare_projected_qkv` does per request
+ * (studio_compute/mlx_decode.py:94-100). For each token and head of q and k:
+ * x <- x / sqrt(mean(x^2) + eps) * weight (where a weight is given), then pair
+ * (i, i + rotary_dim / 2) turns by positions[axis[i]][token] * f_i. All in fp32
+ * (the angle in double), rounded to bf16 once.
+ * q [ntok, Hq, D], k, v [ntok, Hkv, D] bf16, each contiguous along D;
+ * strides       host array of 6: token and head strides (elements) of q, k, v
+ *               (any; 16-byte accesses where all are multiples of 8 and the
+ *               pointers 16-byte aligned)
+ * positions     [axes][ntok] int32, pos_axis_stride elements between axes
+ * turns         [rotary_dim / 2] double: f_i / (2 pi); axis [rotary_dim / 2] int32
+ * q_weight, k_weight [D] bf16 or NULL (no norm), 16-byte aligned
+ * q_out [ntok, Hq, D]; exactly one of k_out [ntok, Hkv, D] (v, slot_mapping
+ * ignored) and kv_pool (k and v written as sc_kv_append does)
+ * Supported: D in {64, 128, 256}, rotary_dim a multiple of 16 in [16, D]. */
+int sc_rotary_append(const sc_bf16* q, const sc_bf16* k, const sc_bf16* v,
+                     const int64_t* strides, const int32_t* positions,
+                     int64_t pos_axis_stride, int axes, const double* turns,
+                     const int32_t* axis, const sc_bf16* q_weight, const sc_bf16* k_weight,
+                     float eps, sc_bf16* q_out, sc_bf16* k_out, sc_bf16* kv_pool,
+                     const int64_t* slot_mapping, int ntok, int Hq, int Hkv, int D,
+                     int rotary_dim, int P, int64_t num_pages, void* stream);
+
+/* The n best continuations over a group's beams and the vocabulary.
+ *
+ * score(k, v) = scores[k] + ((x - m_k) - log sum e^(x - m_k)), m_k = max of row k, in
+ * fp32; ordered by score, equal ones by the lower k * vocab + v. NaN counts as -inf.
+ * logits        [groups * beams] rows of vocab values, row_stride elements apart,
+ *               bf16 (logits_fp32 = 0) or fp32
+ * scores        [groups, beams] fp32 (-inf: a dead beam)
+ * finished      [groups, beams] uint8 or NULL: a nonzero beam's only continuation
+ *               is (pad_token, scores[k])
+ * out_scores, parents, tokens [groups, n]; where fewer than n scores are above
+ *               -inf, the entries of lowest index follow with -inf
+ * workspace     sc_beam_select_workspace bytes, 256-byte aligned
+ * Supported: beams <= 64, n <= 64, beams * vocab < 2^31, groups * beams <= 65535. */
+size_t sc_beam_select_workspace(int groups, int beams, int vocab, int logits_fp32);
+int sc_beam_select(const void* logits, int logits_fp32, int64_t row_stride, const float* scores,
+                   const uint8_t* finished, int pad_token, float* out_scores, int32_t* parents,
+                   int32_t* tokens, void* workspace, size_t workspace_bytes, int groups,
+                   int beams, int vocab, int n, void* stream);
+
+/* State rows follow their beams, in place.
+ *
+ * Pool i is [layers[i]][rows][row_bytes[i]] (16-byte aligned, row_bytes a multiple of
+ * 16; at most 4 pools; the three arrays are host memory). Beam k of group g holds row
+ * slots[g][k]; child j continues beam parents[g][j]. The first child of a beam keeps
+ * its row; each later child takes, in ascending order, the row of a beam without
+ * children, and the parent's row is copied there in every layer of every pool.
+ * slots, parents, new_slots [groups, beams] int32 (slots distinct); copies: scratch of
+ * 2 + 2 * groups * beams int32, 8-byte aligned. A parent outside [0, beams) or a slot
+ * outside [0, rows) is flagged (DEV_BAD_INDEX), and nothing is copied for it. beams <= 64. */
+int sc_reorder_rows(void* const* pools, const int64_t* row_bytes, const int* layers, int npools,
+                    int rows, const int32_t* slots, const int32_t* parents, int32_t* new_slots,
+                    int32_t* copies, int groups, int beams, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

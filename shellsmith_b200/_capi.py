@@ -63,10 +63,17 @@ SIGNATURES = {
                                         _I, _I, _I, _F, _P, _P, _P, _P, _P, _P, _I, _P],
     "sc_paged_decode_attention_noalloc": [_P, _P, _I64, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I,
                                           _F, _P, _P, _P],
+    "sc_rotary_append": [_P, _P, _P, _P, _P, _I64, _I, _P, _P, _P, _P, _F, _P, _P, _P, _P, _I,
+                         _I, _I, _I, _I, _I, _I64, _P],
+    "sc_beam_select_workspace": [_I, _I, _I, _I],
+    "sc_beam_select": [_P, _I, _I64, _P, _P, _I, _P, _P, _P, _P, ctypes.c_size_t, _I, _I, _I, _I,
+                       _P],
+    "sc_reorder_rows": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _I, _I, _P],
 }
 
 
-RESTYPES = {"sc_gdn_decode_glue_workspace": ctypes.c_size_t}
+RESTYPES = {"sc_gdn_decode_glue_workspace": ctypes.c_size_t,
+            "sc_beam_select_workspace": ctypes.c_size_t}
 
 
 class ShellcacheError(RuntimeError):

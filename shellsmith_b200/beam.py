@@ -1,0 +1,124 @@
+"""Beam selection and the reordering of per-sequence state rows (device side).
+
+The reference samples one token per request (studio_compute/inference.py:176-218);
+several beams over one cache also need, after each step,
+
+  beam_select    the best continuations over a group's beams and the vocabulary
+  reorder_rows   state rows (GDN state, conv taps) that follow their beams
+
+Both run on the device without a synchronisation: parents and new slots go from one
+call to the next as tensors. plan_reorder is the same slot rule on the host, for the
+page tables (engine.HybridCacheEngine.reorder).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import torch
+
+from . import _capi
+from ._torch import ptr, require_cuda, stream_of
+
+MAX_BEAMS = 64   # beams of one group
+MAX_SELECT = 64  # continuations asked for at once
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, *,
+                finished: torch.Tensor | None = None, pad_token: int = 0) -> tuple:
+    """The n best continuations of each group's beams.
+
+    logits [G, K, V] bf16 or fp32 (contiguous along V, rows evenly spaced), scores
+    [G, K] fp32 the beams' summed log-probabilities (-inf: the beam is dead). The score
+    of token v after beam k is scores[k] + log_softmax(logits[k])[v] in fp32; the result
+    is ordered by score, equal ones by the lower beam, then the lower token. finished
+    [G, K] bool: such a beam's only continuation is pad_token, its score unchanged.
+    Returns (scores fp32, parents int32, tokens int32), each [G, n]. Where fewer than n
+    continuations have a score above -inf, those of lowest index follow with -inf (a NaN
+    score counts as -inf).
+    """
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 3:
+        raise ValueError("beam_select: logits must be a [groups, beams, vocab] tensor")
+    if not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor (the product path has no CPU fallback)")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"logits must be bfloat16 or float32, got {logits.dtype}")
+    groups, beams, vocab = logits.shape
+    if not (logits.is_contiguous() or groups == 0
+            or (logits.stride(2) == 1 and logits.stride(1) >= vocab
+                and (groups == 1 or logits.stride(0) == beams * logits.stride(1)))):
+        raise ValueError("beam_select: logits need a contiguous vocabulary and evenly spaced rows")
+    require_cuda("scores", scores, torch.float32, 2, align=4)
+    if tuple(scores.shape) != (groups, beams):
+        raise ValueError(f"scores must be [{groups}, {beams}], got {tuple(scores.shape)}")
+    if finished is not None:
+        require_cuda("finished", finished, torch.bool, 2, align=1)
+        if tuple(finished.shape) != (groups, beams):
+            raise ValueError(f"finished must be [{groups}, {beams}], got {tuple(finished.shape)}")
+    if beams < 1 or vocab < 1:
+        raise ValueError("beam_select: at least one beam and one token")
+    fp32 = int(logits.dtype == torch.float32)
+    need = _capi.lib().sc_beam_select_workspace(groups, beams, vocab, fp32)
+    device = logits.device
+    work = torch.empty(need, dtype=torch.uint8, device=device)
+    best = torch.empty((groups, n), dtype=torch.float32, device=device)
+    where = torch.empty((2, groups, n), dtype=torch.int32, device=device)
+    parents, tokens = where[0], where[1]
+    stride = logits.stride(1) if beams > 1 else (logits.stride(0) if groups > 1 else vocab)
+    _capi.call("sc_beam_select", ptr(logits), fp32, max(stride, vocab), ptr(scores), ptr(finished),
+               int(pad_token), ptr(best), ptr(parents), ptr(tokens), ptr(work), need, groups, beams,
+               vocab, int(n), stream_of(logits))
+    return best, parents, tokens
+
+
+def reorder_rows(pools, slots: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
+    """Let each group's state rows follow their beams, in place; returns the new slots.
+
+    pools: up to four contiguous tensors [layers, rows, ...] (any type, rows of a
+    multiple of 16 bytes); beam k of group g holds row slots[g, k] of every layer (all
+    slots distinct). Child j continues beam parents[g, j]: the first child of a beam
+    keeps the beam's row, each later child gets a copy in the row of a beam without
+    children (ascending), so nothing else moves. slots, parents, result: int32 [G, K].
+    """
+    require_cuda("slots", slots, torch.int32, 2, align=4)
+    require_cuda("parents", parents, torch.int32, 2, align=4)
+    if slots.shape != parents.shape:
+        raise ValueError("reorder_rows: slots and parents must have the same shape")
+    groups, beams = slots.shape
+    pools = list(pools)
+    if len(pools) > 4:
+        raise ValueError(f"reorder_rows: at most 4 pools, got {len(pools)}")
+    rows = None
+    for i, pool in enumerate(pools):
+        if not isinstance(pool, torch.Tensor) or not pool.is_cuda or pool.dim() < 2:
+            raise ValueError(f"reorder_rows: pool {i} must be a CUDA tensor [layers, rows, ...]")
+        if not pool.is_contiguous():
+            raise ValueError(f"reorder_rows: pool {i} must be contiguous")
+        if rows not in (None, pool.shape[1]):
+            raise ValueError("reorder_rows: every pool must have the same rows")
+        rows = pool.shape[1]
+    count = len(pools)
+    bases = (ctypes.c_void_p * 4)(*(p.data_ptr() for p in pools))
+    sizes = (ctypes.c_int64 * 4)(*(p.stride(1) * p.element_size() for p in pools))
+    layers = (ctypes.c_int * 4)(*(p.shape[0] for p in pools))
+    out = torch.empty_like(slots)
+    work = torch.empty(2 + 2 * slots.numel(), dtype=torch.int32, device=slots.device)
+    _capi.call("sc_reorder_rows", bases, sizes, layers, count, rows or 1, ptr(slots), ptr(parents),
+               ptr(out), ptr(work), groups, max(beams, 1), stream_of(slots))
+    return out
+
+
+def plan_reorder(slots, parents) -> tuple:
+    """reorder_rows' slot rule for one group on the host: (new slots, [(source, destination)])."""
+    slots, parents = [int(s) for s in slots], [int(p) for p in parents]
+    free = [slots[b] for b in range(len(slots)) if b not in set(parents)]
+    new, copies, seen = [], [], set()
+    for p in parents:
+        if p in seen:
+            copies.append((slots[p], free.pop(0)))
+            new.append(copies[-1][1])
+        else:
+            new.append(slots[p])
+        seen.add(p)
+    return np.asarray(new, np.int64), copies
