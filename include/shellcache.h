@@ -511,6 +511,36 @@ int sc_rotary_append(const sc_bf16* q, const sc_bf16* k, const sc_bf16* v,
                      const int64_t* slot_mapping, int ntok, int Hq, int Hkv, int D,
                      int rotary_dim, int P, int64_t num_pages, void* stream);
 
+/* Split-K decode attention of sequences that share the pages of a long prefix.
+ *
+ * The result of sc_paged_decode_attention; the pages that a group's members share are
+ * read once for up to 128 (member, query head of a kv head) rows instead of once a
+ * member. No reference counterpart (the reference attends one request at a time).
+ *
+ * prefix_pages  [B] int32: leading pages of each sequence attended in its group (0: none)
+ * tiles         [ntiles][4] int32, 16-byte aligned: the first entry of `members`, their
+ *               number (times Hq / Hkv at most 128), their shared pages, and the row
+ *               whose block table lists those pages
+ * members       rows of the batch, each with prefix_pages > 0 in exactly one tile
+ * prefix_pages_per_split, prefix_splits  the split of the shared pages
+ * pages_per_split, num_splits  the split of each sequence's other pages
+ * prefix_out [B, Hq, prefix_splits, D], prefix_lse [B, Hq, prefix_splits], part_out
+ * [B, Hq, num_splits, D], part_lse [B, Hq, num_splits]: fp32 scratch
+ * ctx_len may end inside the shared pages; 0 gives zeros and lse = -inf. q, kv_pool,
+ * out, prefix_out, part_out 16-byte aligned; other arguments, the flagging of bad
+ * indices and the bf16 rounding of the probabilities as in sc_paged_decode_attention.
+ * Supported: D in {64, 128, 256}, P == 16, Hq / Hkv <= 128, prefix_splits + num_splits
+ * <= 1024, num_pages * Hkv * 2 < 2^31. */
+int sc_shared_prefix_attention(const sc_bf16* q, const sc_bf16* kv_pool, int64_t num_pages,
+                               const int32_t* block_table, const int32_t* ctx_len,
+                               const int32_t* seq_order, const int32_t* prefix_pages,
+                               const int32_t* tiles, const int32_t* members, int ntiles, int B,
+                               int Hq, int Hkv, int D, int P, int max_pages,
+                               int prefix_pages_per_split, int prefix_splits,
+                               int pages_per_split, int num_splits, float scale,
+                               float* prefix_out, float* prefix_lse, float* part_out,
+                               float* part_lse, sc_bf16* out, float* lse_out, void* stream);
+
 /* The n best continuations over a group's beams and the vocabulary.
  *
  * score(k, v) = scores[k] + ((x - m_k) - log sum e^(x - m_k)), m_k = max of row k, in

@@ -12,6 +12,8 @@ block manager hands out pages, and these functions move and read them:
   paged_decode_attention  split-K attention of one query per sequence over
                           its ragged pages, then the (out, lse) combine
   attention_combine       merge per-part (out, lse), e.g. across GPUs
+  shared_prefix_attention decode attention of sequences that share the pages of a
+                          prefix, read once for a group (PrefixGroups)
 
 8-bit pools (cache_precision "8bit"): uint8 [num_pages, Hkv, 34 * D], one
 quantised block per (page, kv head) (new_pool_q8); kv_append, kv_copy_pages
@@ -404,6 +406,151 @@ def append_and_attend(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
                                   max_pages_in_batch=max_pages_in_batch,
                                   pages_per_split=pages_per_split, total_pages=total_pages,
                                   workspace=workspace, out=out, seq_order=seq_order, sms=sms)
+
+
+PREFIX_ROWS = 128  # (sequence, query head) rows of one kv head attended together
+
+
+class PrefixGroups:
+    """Which sequences share the pages of a prefix, laid out once for a batch.
+
+    groups: [(rows, prefix_tokens)]: batch rows whose block tables start with the same
+    pages for prefix_tokens tokens (whole pages count; forks of one snapshot share
+    them). Rows in no group, and groups of one row, attend as in
+    paged_decode_attention. The plan holds while the groups do: contexts may grow.
+    """
+
+    def __init__(self, groups, batch: int, q_heads: int, kv_heads: int, head_dim: int,
+                 device: str | torch.device = "cuda", sms: int | None = None):
+        if q_heads % kv_heads or q_heads // kv_heads > PREFIX_ROWS:
+            raise ValueError(f"PrefixGroups: {q_heads} query heads over {kv_heads} kv heads")
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"PrefixGroups: head_dim must be 64, 128 or 256, got {head_dim}")
+        self.batch, self.q_heads, self.kv_heads, self.head_dim = batch, q_heads, kv_heads, head_dim
+        per_tile = PREFIX_ROWS // (q_heads // kv_heads)
+        first_page, tiles, members = [0] * batch, [], []
+        seen: set = set()
+        for rows, tokens in groups:
+            rows, pages = [int(r) for r in rows], int(tokens) // PAGE_SIZE
+            if any(r < 0 or r >= batch or r in seen for r in rows) or len(set(rows)) < len(rows):
+                raise ValueError("PrefixGroups: a row is outside the batch or in two groups")
+            if tokens < 0:
+                raise ValueError(f"PrefixGroups: a prefix of {tokens} tokens")
+            seen.update(rows)
+            if len(rows) < 2 or pages == 0:
+                continue
+            count = -(-len(rows) // per_tile)
+            for i in range(count):  # even tiles
+                part = rows[len(rows) * i // count:len(rows) * (i + 1) // count]
+                tiles.append((len(members), len(part), pages, part[0]))
+                members += part
+            for r in rows:
+                first_page[r] = pages
+        self.ntiles = len(tiles)
+        self.max_prefix_pages = max((t[2] for t in tiles), default=0)
+        self.min_first_page = min(first_page, default=0)
+        self.pages_per_split, self.num_splits = prefix_split_plan(
+            [t[2] for t in tiles], kv_heads, head_dim, sms or sm_count(device))
+        # One transfer: tiles [ntiles, 4], then first_page [batch], then members.
+        flat = torch.tensor([x for t in tiles for x in t] + first_page + members,
+                            dtype=torch.int32).to(device)
+        self.tiles = flat[:4 * len(tiles)]
+        self.first_page = flat[4 * len(tiles):4 * len(tiles) + batch]
+        self.members = flat[4 * len(tiles) + batch:]
+
+
+def prefix_split_plan(tile_pages: list, kv_heads: int, head_dim: int, sms: int) -> tuple:
+    """(pages_per_split, num_splits) of the shared pages: about one CTA per SM over all
+    tiles and kv heads, in whole tiles of the kernel (4 pages at D = 256, else 8)."""
+    unit = 4 if head_dim == 256 else 8
+    work = sum(tile_pages) * kv_heads
+    pps = max(unit, -(-work // (sms * unit)) * unit)
+    return pps, max(1, -(-max(tile_pages, default=1) // pps))
+
+
+class SharedPrefixWorkspace:
+    """Reusable scratch of shared_prefix_attention (the partials); grows when needed."""
+
+    def __init__(self, device: str | torch.device = "cuda"):
+        self.device = torch.device(device)
+        self._buffer = torch.empty(0, dtype=torch.float32, device=device)
+
+    def parts(self, rows: int, dim: int, prefix_splits: int, splits: int) -> tuple:
+        """Addresses of prefix_out, prefix_lse, part_out, part_lse for `rows` (row, head)s."""
+        sizes = [-(-n // 4) * 4 for n in (rows * prefix_splits * dim, rows * prefix_splits,
+                                          rows * splits * dim, rows * splits)]
+        if self._buffer.numel() < sum(sizes):
+            self._buffer = torch.empty(sum(sizes), dtype=torch.float32, device=self.device)
+        at = self._buffer.data_ptr()
+        out = []
+        for n in sizes:
+            out.append(at)
+            at += 4 * n
+        return tuple(out)
+
+
+def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tensor,
+                            ctx_len: torch.Tensor, scale: float, groups: PrefixGroups, *,
+                            max_suffix_pages: int | None = None,
+                            total_suffix_pages: int | None = None,
+                            workspace: SharedPrefixWorkspace | None = None,
+                            out: torch.Tensor | None = None,
+                            lse_out: torch.Tensor | None = None,
+                            seq_order: torch.Tensor | None = None,
+                            sms: int | None = None) -> torch.Tensor:
+    """paged_decode_attention where groups of sequences share the pages of a prefix: these
+    are read once for a group (tensor cores, up to 128 (sequence, head) rows together).
+
+    max_suffix_pages / total_suffix_pages (host-known): the most pages any sequence has
+    past its shared ones, and their sum over the batch (whole sequences where there is no
+    group); when omitted the block-table width bounds them. seq_order as in
+    paged_decode_attention. lse_out [B * Hq] fp32. bf16 pools only.
+    """
+    if kv_pool.dtype != torch.bfloat16:
+        raise TypeError("shared_prefix_attention takes bf16 pools")
+    num_pages, hkv, page, dim = _pool_dims(kv_pool)
+    require_cuda("q", q, torch.bfloat16, 3)
+    require_cuda("block_table", block_table, torch.int32, 2, align=4)
+    require_cuda("ctx_len", ctx_len, torch.int32, 1, align=4)
+    B, hq, d = q.shape
+    if d != dim or hq % hkv or block_table.shape[0] != B or ctx_len.shape[0] != B:
+        raise ValueError("shared_prefix_attention: inconsistent shapes")
+    if (groups.batch, groups.q_heads, groups.kv_heads, groups.head_dim) != (B, hq, hkv, dim):
+        raise ValueError("shared_prefix_attention: the groups were laid out for another batch")
+    max_pages = block_table.shape[1]
+    if groups.max_prefix_pages > max_pages:
+        raise ValueError("shared_prefix_attention: a prefix is longer than the block table")
+    if groups.ntiles == 0:
+        return paged_decode_attention(q, kv_pool, block_table, ctx_len, scale,
+                                      max_pages_in_batch=max_suffix_pages,
+                                      total_pages=total_suffix_pages, out=out, lse_out=lse_out,
+                                      seq_order=seq_order, sms=sms)
+    pps, nsplit = decode_plan(B, hq, hkv, max_suffix_pages or max_pages, None,
+                              total_suffix_pages, sms or sm_count(q.device))
+    if out is None:
+        out = torch.empty((B, hq, dim), dtype=torch.bfloat16, device=q.device)
+    else:
+        require_cuda("out", out, torch.bfloat16, 3)
+        if out.shape != q.shape:
+            raise ValueError("shared_prefix_attention: out must have q's shape")
+    if lse_out is not None:
+        require_cuda("lse_out", lse_out, torch.float32, 1, align=4)
+        if lse_out.shape[0] != B * hq:
+            raise ValueError("shared_prefix_attention: lse_out must be [B * Hq]")
+    if seq_order is not None:
+        require_cuda("seq_order", seq_order, torch.int32, 1, align=4)
+        if seq_order.shape[0] != B:
+            raise ValueError("shared_prefix_attention: seq_order needs one entry per sequence")
+    if workspace is None:
+        workspace = SharedPrefixWorkspace(q.device)
+    pre_out, pre_lse, part_out, part_lse = workspace.parts(B * hq, dim, groups.num_splits, nsplit)
+    _capi.call("sc_shared_prefix_attention", ptr(q), ptr(kv_pool), num_pages, ptr(block_table),
+               ptr(ctx_len), ptr(seq_order), ptr(groups.first_page), ptr(groups.tiles),
+               ptr(groups.members), groups.ntiles, B, hq, hkv, dim, page, max_pages,
+               groups.pages_per_split, groups.num_splits, pps, nsplit, float(scale), pre_out,
+               pre_lse, part_out, part_lse, ptr(out), ptr(lse_out), stream_of(q))
+    _count(3 if B else 0)
+    return out
 
 
 def attention_combine(part_out: torch.Tensor, part_lse: torch.Tensor,
