@@ -523,9 +523,11 @@ int sc_rotary_append(const sc_bf16* q, const sc_bf16* k, const sc_bf16* v,
  *               whose block table lists those pages
  * members       rows of the batch, each with prefix_pages > 0 in exactly one tile
  * prefix_pages_per_split, prefix_splits  the split of the shared pages
- * pages_per_split, num_splits  the split of each sequence's other pages
+ * pages_per_split (at most 32), num_splits  the split of each sequence's other pages
  * prefix_out [B, Hq, prefix_splits, D], prefix_lse [B, Hq, prefix_splits], part_out
  * [B, Hq, num_splits, D], part_lse [B, Hq, num_splits]: fp32 scratch
+ * counters      ceil(B / 1024) int32 of scratch
+ * Launches that share scratch must not overlap on the GPU.
  * ctx_len may end inside the shared pages; 0 gives zeros and lse = -inf. q, kv_pool,
  * out, prefix_out, part_out 16-byte aligned; other arguments, the flagging of bad
  * indices and the bf16 rounding of the probabilities as in sc_paged_decode_attention.
@@ -533,13 +535,13 @@ int sc_rotary_append(const sc_bf16* q, const sc_bf16* k, const sc_bf16* v,
  * <= 1024, num_pages * Hkv * 2 < 2^31. */
 int sc_shared_prefix_attention(const sc_bf16* q, const sc_bf16* kv_pool, int64_t num_pages,
                                const int32_t* block_table, const int32_t* ctx_len,
-                               const int32_t* seq_order, const int32_t* prefix_pages,
-                               const int32_t* tiles, const int32_t* members, int ntiles, int B,
-                               int Hq, int Hkv, int D, int P, int max_pages,
+                               const int32_t* prefix_pages, const int32_t* tiles,
+                               const int32_t* members, int ntiles, int B, int Hq, int Hkv, int D, int P, int max_pages,
                                int prefix_pages_per_split, int prefix_splits,
                                int pages_per_split, int num_splits, float scale,
                                float* prefix_out, float* prefix_lse, float* part_out,
-                               float* part_lse, sc_bf16* out, float* lse_out, void* stream);
+                               float* part_lse, int32_t* counters, sc_bf16* out, float* lse_out,
+                               void* stream);
 
 /* The n best continuations over a group's beams and the vocabulary.
  *

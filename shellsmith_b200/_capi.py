@@ -65,8 +65,8 @@ SIGNATURES = {
                                           _F, _P, _P, _P],
     "sc_rotary_append": [_P, _P, _P, _P, _P, _I64, _I, _P, _P, _P, _P, _F, _P, _P, _P, _P, _I,
                          _I, _I, _I, _I, _I, _I64, _P],
-    "sc_shared_prefix_attention": [_P, _P, _I64, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
-                                   _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P, _P, _P],
+    "sc_shared_prefix_attention": [_P, _P, _I64, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
+                                   _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P, _P, _P, _P],
     "sc_beam_select_workspace": [_I, _I, _I, _I],
     "sc_beam_select": [_P, _I, _I64, _P, _P, _I, _P, _P, _P, _P, ctypes.c_size_t, _I, _I, _I, _I,
                        _P],

@@ -124,19 +124,11 @@ struct FusedArgs {
   uint16_t* pool = nullptr;
   unsigned int* counters = nullptr;
   int merge = 0;  // 1: the splits merge in the kernel (num_splits <= kFusedMergeParts)
-  const int32_t* first_page = nullptr;  // kTail: pages of each sequence that are left out
 };
 
-// What a launch does beside the split-K attention over whole sequences (kPlain):
-// kFused appends the step's new tokens; kTail attends only to the pages from
-// min(first_page[b], ctx / 16) on, always writes partials, and runs beside the kernel queued before
-// it (shared_prefix.cu: the attention over the prefix pages, whose own wait has seen
-// everything this kernel reads).
-enum DecodeMode : int { kPlainMode = 0, kFusedMode = 1, kTailMode = 2 };
-
-template <int D, int NW, int NSTAGE, int kMode>
-__device__ __forceinline__ void
-    paged_decode_body(const uint16_t* __restrict__ q, const uint16_t* __restrict__ kv_pool,
+template <int D, int NW, int NSTAGE, bool kFused>
+__global__ void __launch_bounds__(NW * 32)
+    paged_decode_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ kv_pool,
                         const int32_t* __restrict__ block_table,
                         const int32_t* __restrict__ ctx_len,
                         const int32_t* __restrict__ seq_order, int Hq, int Hkv, int G, int HG,
@@ -144,11 +136,12 @@ __device__ __forceinline__ void
                         float* __restrict__ part_out, float* __restrict__ part_lse,
                         uint16_t* __restrict__ out, float* __restrict__ lse_out,
                         float* __restrict__ packed, long long num_pages,
-                        unsigned int* status, const FusedArgs& fa) {
+                        unsigned int* status, FusedArgs fa) {
   using S = AttnShape<D>;
-  constexpr bool kFused = kMode == kFusedMode, kTail = kMode == kTailMode;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + NW * NSTAGE * S::STAGE_BYTES);
+  pdl_wait();
+  pdl_trigger();
 
   const int split = blockIdx.x;
   const int kvh = blockIdx.y / HG;
@@ -159,26 +152,13 @@ __device__ __forceinline__ void
     if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) flag_device(status, DEV_BAD_INDEX);
     return;
   }
-  const bool reports = split == 0 && blockIdx.y == 0 && threadIdx.x == 0;
-  int skip = 0, ctx = ctx_len[b];
-  if constexpr (kTail) {
-    skip = fa.first_page[b];
-    if (skip < 0 || skip > max_pages) {
-      if (reports) flag_device(status, DEV_BAD_INDEX);
-      skip = max(0, min(skip, max_pages));
-    }
-    if (ctx >= 0) {  // a page that the context ends in is never left out
-      skip = min(skip, ctx / kPage);
-      ctx -= skip * kPage;
-    }
-  }
-  const int L = checked_ctx_len(ctx, kPage, max_pages - skip, pages_per_split, num_splits, status,
-                                reports);
+  const int L = checked_ctx_len(ctx_len[b], kPage, max_pages, pages_per_split, num_splits,
+                                status, split == 0 && blockIdx.y == 0 && threadIdx.x == 0);
   const int npages = (L + kPage - 1) / kPage;
   const int p_begin = split * pages_per_split;
   // Splits this sequence fills: with one, the CTA writes the final rows itself.
   const int ns_seq = (npages + pages_per_split - 1) / pages_per_split;
-  const bool final_here = !kTail && (num_splits == 1 || (kFused && fa.merge && ns_seq <= 1));
+  const bool final_here = num_splits == 1 || (kFused && fa.merge && ns_seq <= 1);
 
   // The appended token (kFused): its page and offset, and its rows written to
   // the pool once per (sequence, kv head), by split 0 of head group 0. A CTA
@@ -263,7 +243,7 @@ __device__ __forceinline__ void
   const int nj = n_here > warp ? (n_here - warp + NW - 1) / NW : 0;
   uint8_t* stage = smem + warp * NSTAGE * S::STAGE_BYTES;
   uint64_t* bar = bars + warp * NSTAGE;
-  const int32_t* bt_row = block_table + (size_t)b * max_pages + skip;
+  const int32_t* bt_row = block_table + (size_t)b * max_pages;
 
   auto issue = [&](int j) {
     int page = bt_row[p_begin + warp + j * NW];
@@ -472,27 +452,6 @@ __device__ __forceinline__ void
       }
     }
   }
-}
-
-template <int D, int NW, int NSTAGE, int kMode>
-__global__ void __launch_bounds__(NW * 32)
-    paged_decode_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ kv_pool,
-                        const int32_t* __restrict__ block_table,
-                        const int32_t* __restrict__ ctx_len,
-                        const int32_t* __restrict__ seq_order, int Hq, int Hkv, int G, int HG,
-                        int max_pages, int pages_per_split, int num_splits, float scale_log2,
-                        float* __restrict__ part_out, float* __restrict__ part_lse,
-                        uint16_t* __restrict__ out, float* __restrict__ lse_out,
-                        float* __restrict__ packed, long long num_pages,
-                        unsigned int* status, FusedArgs fa) {
-  if constexpr (kMode != kTailMode) pdl_wait();
-  pdl_trigger();
-  paged_decode_body<D, NW, NSTAGE, kMode>(q, kv_pool, block_table, ctx_len, seq_order, Hq, Hkv, G,
-                                          HG, max_pages, pages_per_split, num_splits, scale_log2,
-                                          part_out, part_lse, out, lse_out, packed, num_pages,
-                                          status, fa);
-  // The grid ends after the one before it, so what waits for this one waits for both.
-  if constexpr (kMode == kTailMode) pdl_wait();
 }
 
 // One CTA per output row: merges the partials of that row.
@@ -819,24 +778,22 @@ int launch_decode(const uint16_t* q, const uint16_t* kv_pool, const int32_t* blo
                   int pages_per_split, int num_splits, float scale, float* part_out,
                   float* part_lse, uint16_t* out, float* lse_out, float* packed,
                   long long num_pages, const PeerPut* put, const FusedArgs* fused,
-                  cudaStream_t s, bool tail = false) {
+                  cudaStream_t s) {
   using S = AttnShape<D>;
   constexpr int NW = kWarpsPerCta, NST = kStages;
   const size_t smem = (size_t)NW * NST * S::STAGE_BYTES + NW * NST * sizeof(uint64_t);
-  auto kernel = tail               ? paged_decode_kernel<D, NW, NST, kTailMode>
-                : fused != nullptr ? paged_decode_kernel<D, NW, NST, kFusedMode>
-                                   : paged_decode_kernel<D, NW, NST, kPlainMode>;
-  const int mode = tail ? kTailMode : fused != nullptr ? kFusedMode : kPlainMode;
-  static int configured[3][64] = {};
+  auto kernel = fused != nullptr ? paged_decode_kernel<D, NW, NST, true>
+                                 : paged_decode_kernel<D, NW, NST, false>;
+  static int configured[2][64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !configured[mode][dev]) {
+  if (dev >= 0 && dev < 64 && !configured[fused != nullptr][dev]) {
     cudaError_t err =
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err != cudaSuccess)
       return set_error(SC_ERR_CUDA, "sc_paged_decode_attention: smem attribute: %s",
                        cudaGetErrorString(err));
-    configured[mode][dev] = 1;
+    configured[fused != nullptr][dev] = 1;
   }
   const int G = Hq / Hkv;
   const int HG = (G + kHeadsPerTile - 1) / kHeadsPerTile;
@@ -851,7 +808,6 @@ int launch_decode(const uint16_t* q, const uint16_t* kv_pool, const int32_t* blo
     return set_error(SC_ERR_CUDA, "sc_paged_decode_attention: launch: %s",
                      cudaGetErrorString(err));
   if (int rc = check_launch("sc_paged_decode_attention")) return rc;
-  if (tail) return SC_OK;  // the caller merges the partials with those of the prefix
   if (fused != nullptr && fused->merge) return SC_OK;  // the splits merged themselves
   if (put != nullptr) {  // the entry guarantees num_splits > 1
     dim3 cgrid(B * Hq, (D + 31) / 32);
@@ -870,19 +826,6 @@ int launch_decode(const uint16_t* q, const uint16_t* kv_pool, const int32_t* blo
 }
 
 }  // namespace
-
-int launch_decode_tail(const uint16_t* q, const uint16_t* kv_pool, long long num_pages,
-                       const int32_t* block_table, const int32_t* ctx_len,
-                       const int32_t* seq_order, const int32_t* first_page, int B, int Hq, int Hkv,
-                       int D, int max_pages, int pages_per_split, int num_splits, float scale,
-                       float* part_out, float* part_lse, cudaStream_t s) {
-  FusedArgs fa;
-  fa.first_page = first_page;
-  const auto launch = D == 64 ? launch_decode<64> : D == 128 ? launch_decode<128> : launch_decode<256>;
-  return launch(q, kv_pool, block_table, ctx_len, seq_order, B, Hq, Hkv, max_pages,
-                pages_per_split, num_splits, scale, part_out, part_lse, nullptr, nullptr, nullptr,
-                num_pages, nullptr, &fa, s, true);
-}
 }  // namespace sc
 
 namespace sc {

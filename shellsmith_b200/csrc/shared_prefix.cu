@@ -7,32 +7,45 @@
 // union splits into parts (m, sum, output) that merge exactly, so the prefix is
 // attended once for the whole group and each sequence's own tail by itself:
 //   prefix_kernel        Q of 128 (sequence, head) rows against a split of the prefix
-//   the split-K kernel   one query a sequence against its own pages (paged_attention.cu)
+//   tail_kernel          one query a sequence against its own pages
 //   merge_parts_kernel   the parts of each row -> bf16
-// The first two run side by side (the second does not wait for the first to end).
+// The first two run side by side: the second does not wait for the first to end, and a
+// CTA of each fits on an SM, so that one's loads run under the other's products.
 //
 // B200 mapping of prefix_kernel. Read once for 128 rows, a K/V byte carries 128
 // multiply-adds, too many for the warp tensor path to keep up with HBM: tcgen05.
-// One CTA per (split, kv head, tile of rows) and SM, six warps:
-//   warps 0-3  one row a thread: scores out of TMEM, online softmax, P back into TMEM
-//   warp 4     TMA: page ids from the block table, K and V tiles into rings of stages
-//   warp 5     issues S = Q K^T (Q in TMEM) and O += P V (P in TMEM, over its scores)
-// A stage holds kTok tokens of 16-token pages. The pool's rows are stored with their
-// 16-byte chunks already permuted as the 128-byte swizzle wants them, so each 64-column
-// slice of a page arrives by an unswizzled 16 x 128-byte TMA box and lands as two
-// swizzle atoms; the slices of a tile's pages follow each other, which makes K a
-// K-major and V an MN-major operand without a copy. S is double buffered: the scores of
+// One CTA per (split, kv head, tile of rows) and SM, eleven warps:
+//   warps 0-7  softmax: warp w holds rows 32 (w % 4) .. (its TMEM lanes), one a thread,
+//              and half w / 4 of each tile's columns: scores out of TMEM, P back
+//   warps 8, 9 TMA: page ids from the block table, K (V) tiles into a ring of stages
+//   warp 10    issues S = Q K^T (Q in TMEM) and O += P V (P in TMEM, over its scores)
+// A stage holds the pages of TOK tokens. The pool's rows are stored with their 16-byte
+// chunks already permuted as the 128-byte swizzle wants them, so an unswizzled TMA box
+// (8 or 16 tokens x 64 columns x D / 64 slices) lands as swizzle atoms and nothing is
+// copied. K comes in boxes of half a page: its 8-token groups are then evenly spaced and
+// one product covers the tile's tokens. V comes in boxes of a page, the 16 rows of one
+// step of its product. The whole MMA warp walks the loop and one elected lane issues: its
+// operands stay in uniform registers (a product of N = 64 then takes 32 cycles; issued
+// from a lane's own branch it took 49). S is double buffered: the scores of
 // tile i + 1 are made while the softmax of tile i runs. O stays in TMEM and is rescaled
 // only when a row's maximum grows by more than 2^8 over its reference (until then P may
 // be as large as 2^8, which costs fp32 sums and bf16 P no accuracy).
 // P is rounded to bf16 for the tensor cores, as in the split-K kernel; scores, maxima,
-// sums and O are fp32.
+// sums and O are fp32. Two stages (128 KB at D = 256) leave room for the tail's CTA.
+//
+// tail_kernel. HBM-bound, 8 query heads to a K/V byte: the warp tensor path is enough.
+// Every warp is on its own: it takes a unit of work (a sequence, a kv head's group of up
+// to 8 query heads, a chunk of pages_per_split pages) off a counter, streams the unit's
+// pages through three stages with one bulk copy a page and writes the unit's partial from
+// its registers. The next unit is taken and its first pages are ordered while the present
+// one is computed, so the stream does not break between units. Scores are transposed,
+// S^T[token, head] = K Q^T (M = 16 tokens = a page, N = 8 heads), and O^T += V^T P^T.
 #include <cudaTypedefs.h>
 #include <math_constants.h>
 
+#include <algorithm>
 #include <mutex>
 
-#include "attention_internal.cuh"
 #include "tc.cuh"
 
 namespace sc {
@@ -40,18 +53,23 @@ namespace {
 
 constexpr int kPageTok = 16;
 constexpr int kRowsTile = 128;
-constexpr int kSoftWarps = 4;
-constexpr int kPrefixThreads = 192;
+constexpr int kSoftThreads = 256;
+constexpr int kTmaWarp = 8, kMmaWarp = 10;  // kTmaWarp: K, the next one: V
+constexpr int kPrefixThreads = 352;
+constexpr int kSoftBar = 1;      // named barrier of the softmax warps
 constexpr float kRescale = 8.f;  // log2 units
 
 template <int D>
 struct PrefixShape {
   static constexpr int TOK = D == 256 ? 64 : 128;  // tokens of a tile
   static constexpr int PAGES = TOK / kPageTok;
-  static constexpr int SEGS = D / 64;              // 128-byte column slices
+  static constexpr int PAGE_BYTES = kPageTok * D * 2;  // K or V of a page
   static constexpr int TILE_BYTES = TOK * D * 2;   // K or V
-  static constexpr int STAGES = 98304 / TILE_BYTES;
-  static constexpr int SMEM = 2 * STAGES * TILE_BYTES + 1024 + 512;
+  static constexpr int STAGES = 65536 / TILE_BYTES;
+  static constexpr int SMEM = 2 * STAGES * TILE_BYTES + 2 * kRowsTile * 4 + 256;
+  // The partials leave through shared memory, kPiece columns of a thread's row at a time.
+  static constexpr int PIECE = D == 64 ? 32 : 64, PITCH = PIECE * 4 + 16;
+  static_assert(kSoftThreads * PITCH <= 2 * STAGES * TILE_BYTES, "epilogue staging");
   // TMEM columns: O, Q (two bf16 a column), two score buffers.
   static constexpr int T_Q = D, T_S = D + D / 2;
   static_assert(T_S + 2 * TOK <= 512, "TMEM plan");
@@ -65,9 +83,10 @@ struct PrefixArgs {
   const int4* tiles;        // first member, members, prefix pages, leader row
   const int32_t* members;   // rows of the batch
   float *part_out, *part_lse;
+  int* counters;            // the tail's work counters, one per slab of rows
   long long num_pages;
   float scale_log2;
-  int B, Hq, Hkv, G, max_pages, pages_per_split, num_splits;
+  int B, Hq, Hkv, G, max_pages, pages_per_split, num_splits, slabs;
   unsigned int* status;
 };
 
@@ -91,14 +110,61 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
+}
+
+// tc::mma_bf16_ts on the lane with `elected` set, from converged code.
+__device__ __forceinline__ void mma_elected(uint32_t elected, uint32_t d_tmem, uint32_t a_tmem,
+                                            uint64_t b_desc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      :
+      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u),
+        "r"(elected)
+      : "memory");
+}
+
+// Barrier of the softmax warps that ORs a predicate over them.
+__device__ __forceinline__ bool soft_any(bool pred) {
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((int)pred), "r"(kSoftBar), "r"(kSoftThreads)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void soft_sync() {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(kSoftBar), "r"(kSoftThreads) : "memory");
+}
+
+// 112 registers: three of the eleven warps share a quarter of the SM's registers with a
+// warp of the tail kernel (168 at D = 256), or no tail CTA would fit beside this one.
 template <int D>
-__global__ void __launch_bounds__(kPrefixThreads, 1)
-    prefix_kernel(const __grid_constant__ CUtensorMap pool, const PrefixArgs a) {
+__global__ void __maxnreg__(112)
+    prefix_kernel(const __grid_constant__ CUtensorMap half_pages,
+                  const __grid_constant__ CUtensorMap whole_pages, const PrefixArgs a) {
   using S = PrefixShape<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                           ~uintptr_t(1023));
-  uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + 2 * S::STAGES * S::TILE_BYTES);
+  // All shared memory is dynamic: it then starts at a multiple of 1024 bytes, as the
+  // swizzled tiles need, and there is no room on the SM for slack beside a tail CTA.
+  extern __shared__ __align__(1024) uint8_t sm[];
+  float(*s_half)[kRowsTile] =  // a row's value of each column half
+      reinterpret_cast<float(*)[kRowsTile]>(sm + 2 * S::STAGES * S::TILE_BYTES);
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(s_half + 2);
   uint64_t* vfull = kfull + S::STAGES;
   uint64_t* kfree = vfull + S::STAGES;
   uint64_t* vfree = kfree + S::STAGES;
@@ -107,40 +173,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   uint64_t* ofull = pfull + 2;          // [2] O has taken it
   uint64_t* qfull = ofull + 2;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(qfull + 1);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int& s_pages = *reinterpret_cast<int*>(s_tmem + 1);
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
   const int split = blockIdx.x, kvh = blockIdx.y;
-  pdl_wait();
-  pdl_trigger();
-
-  const int4 tile = a.tiles[blockIdx.z];
-  const int p0 = split * a.pages_per_split;
-  if (p0 >= tile.z) return;  // uniform over the CTA
-  if (tile.w < 0 || tile.w >= a.B || tile.z > a.max_pages || tile.y * a.G > kRowsTile) {
-    if (tid == 0) flag_device(a.status, DEV_BAD_INDEX);
-    return;
-  }
-  // A member attends here to the whole pages of its context; a page that its context
-  // ends in is its tail's. Pages that no member attends to are not read.
-  const auto pages_of = [&](int b) { return min(tile.z, max(a.ctx_len[b], 0) / kPageTok); };
-  __shared__ int s_pages;
-  if (tid == 0) s_pages = 0;
-  __syncthreads();
-  if (tid < tile.y) {
-    const int b = a.members[tile.x + tid];
-    if (b >= 0 && b < a.B)
-      atomicMax(&s_pages, pages_of(b));
-    else
-      flag_device(a.status, DEV_BAD_INDEX);
-  }
-  __syncthreads();
-  const int npages = min(p0 + a.pages_per_split, s_pages) - p0;
-  if (npages <= 0) return;
-  if (a.status != nullptr &&
-      (*reinterpret_cast<volatile unsigned int*>(a.status) & DEV_WAIT_TIMEOUT))
-    return;
-  const int ntiles = (npages + S::PAGES - 1) / S::PAGES;
-
   if (tid == 0) {
+    s_pages = 0;
     for (int i = 0; i < S::STAGES; ++i) {
       mbar_init(&kfull[i], 1);
       mbar_init(&vfull[i], 1);
@@ -149,32 +187,77 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sfull[i], 1);
-      mbar_init(&pfull[i], kSoftWarps * 32);
+      mbar_init(&pfull[i], kSoftThreads);
       mbar_init(&ofull[i], 1);
     }
-    mbar_init(qfull, kSoftWarps * 32);
+    mbar_init(qfull, kSoftThreads);
     fence_mbar_init();
   }
-  if (warp == 5) tc::tmem_alloc(s_tmem, 512);
+  pdl_wait();
+  if (tid == 0 && blockIdx.x + blockIdx.y + blockIdx.z == 0) {
+    // The tail starts once every CTA has triggered; its counters are zero by then.
+    for (int i = 0; i < a.slabs; ++i) atomicExch(a.counters + i, 0);
+    __threadfence();
+  }
+  __syncthreads();
+  pdl_trigger();
+
+  const int4 tile = a.tiles[blockIdx.z];
+  const int p0 = split * a.pages_per_split;
+  if (p0 >= tile.z) return;  // uniform over the CTA
+  if (smem_addr(sm) & 1023u) {  // never seen; better void than wrong
+    if (tid == 0) flag_device(a.status, DEV_WAIT_TIMEOUT);
+    return;
+  }
+  if (tile.w < 0 || tile.w >= a.B || tile.z > a.max_pages || tile.y * a.G > kRowsTile) {
+    if (tid == 0) flag_device(a.status, DEV_BAD_INDEX);
+    return;
+  }
+  // A member attends here to the whole pages of its context; a page that its context
+  // ends in is its tail's. Pages that no member attends to are not read.
+  const auto pages_of = [&](int b) { return min(tile.z, max(a.ctx_len[b], 0) / kPageTok); };
+  if (tid < tile.y) {
+    const int b = a.members[tile.x + tid];
+    if (b >= 0 && b < a.B)
+      atomicMax(&s_pages, pages_of(b));
+    else
+      flag_device(a.status, DEV_BAD_INDEX);
+  }
+  const bool stop = a.status != nullptr &&
+                    (*reinterpret_cast<volatile unsigned int*>(a.status) & DEV_WAIT_TIMEOUT);
+  // After a bounded wait has given up on this device, later CTAs stop at once.
+  if (__syncthreads_or(stop)) return;
+  const int npages = min(p0 + a.pages_per_split, s_pages) - p0;
+  if (npages <= 0) return;
+  const int ntiles = (npages + S::PAGES - 1) / S::PAGES;
+  if (warp == kMmaWarp) tc::tmem_alloc(s_tmem, 512);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *s_tmem;
 
-  if (warp == 4) {
+  // Every wait is bounded. After one has given up (the status word says so) a role runs
+  // on without waiting, so that the others' barriers still complete; the results are void.
+  bool ok = true;
+  const auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (ok) ok = mbar_wait_bounded(bar, parity, a.status);
+  };
+
+  if (warp == kTmaWarp || warp == kTmaWarp + 1) {
     // ---------------------------------------------------------------- TMA
-    // Lane l moves slice l % SEGS of page l / SEGS of the tile, K and then V.
+    // One box a lane: half pages of K, pages of V.
+    const int which = warp - kTmaWarp;
     const int32_t* row = a.block_table + (size_t)tile.w * a.max_pages + p0;
-    constexpr int kBoxes = S::PAGES * S::SEGS;  // 16 for every D
-    static_assert(kBoxes == 16 || kBoxes == 8, "one box a lane, K on one half, V on the other");
-    const int box = lane & 15, which = lane >> 4;
-    const bool moves = box < kBoxes;
-    const int pg = box / S::SEGS, seg = box % S::SEGS;
+    const int boxes = which ? S::PAGES : 2 * S::PAGES;
+    const int box_bytes = which ? S::PAGE_BYTES : S::PAGE_BYTES / 2;
+    const int pg = which ? lane : lane >> 1;
+    const bool moves = lane < boxes;
+    uint64_t *full = which ? vfull : kfull, *freed = which ? vfree : kfree;
+    const CUtensorMap* map = which ? &whole_pages : &half_pages;
     const auto page_of = [&](int i) {  // pages past the end repeat the last one (masked)
       return moves && i < ntiles ? row[min(i * S::PAGES + pg, npages - 1)] : 0;
     };
     int page = page_of(0);
-    int issued = 0;
     for (int i = 0; i < ntiles; ++i) {
       const int next = page_of(i + 1);
       const int st = i % S::STAGES, round = i / S::STAGES;
@@ -182,91 +265,92 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         flag_device(a.status, DEV_BAD_INDEX);
         page = 0;  // keep the copy in bounds; the status word reports the fault
       }
-      bool ok = true;
-      if (lane == 0 && round > 0)
-        ok = mbar_wait_bounded(&kfree[st], (round - 1) & 1, a.status) &&
-             mbar_wait_bounded(&vfree[st], (round - 1) & 1, a.status);
-      if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&kfull[st], S::TILE_BYTES);
-        mbar_arrive_expect_tx(&vfull[st], S::TILE_BYTES);
-      }
+      if (i >= S::STAGES) wait(&freed[st], (round - 1) & 1);
+      if (lane == 0) mbar_arrive_expect_tx(&full[st], S::TILE_BYTES);
       __syncwarp();
-      if (moves) {
-        const uint32_t dst = smem_addr(sm + (which * S::STAGES + st) * S::TILE_BYTES) +
-                             seg * (S::TOK * 128) + pg * (kPageTok * 128);
-        tma_load_4d(dst, &pool, 0, 0, seg, (page * a.Hkv + kvh) * 2 + which,
-                    which ? &vfull[st] : &kfull[st]);
-      }
-      issued = i + 1;
+      if (moves)
+        tma_load_4d(smem_addr(sm + (which * S::STAGES + st) * S::TILE_BYTES + lane * box_bytes),
+                    map, 0, which ? 0 : 8 * (lane & 1), 0, (page * a.Hkv + kvh) * 2 + which,
+                    &full[st]);
       page = next;
     }
+    __syncwarp();
     // The last copy into each stage has landed before the CTA ends.
+    ok = true;
     if (lane == 0)
-      for (int i = max(0, issued - S::STAGES); i < issued; ++i) {
-        mbar_wait_bounded(&kfull[i % S::STAGES], (i / S::STAGES) & 1, a.status);
-        mbar_wait_bounded(&vfull[i % S::STAGES], (i / S::STAGES) & 1, a.status);
-      }
-  } else if (warp == 5) {
+      for (int i = max(0, ntiles - S::STAGES); i < ntiles; ++i)
+        wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
+  } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- MMA
-    if (lane == 0) {
-      constexpr uint32_t kIdS = tc::idesc_bf16(kRowsTile, S::TOK, false, false);
-      constexpr uint32_t kIdO = tc::idesc_bf16(kRowsTile, D, false, true);
-      const auto scores = [&](int i) {
-        const int st = i % S::STAGES;
-        if (!mbar_wait_bounded(&kfull[st], (i / S::STAGES) & 1, a.status)) return false;
-        tc::fence_after();
-        const uint32_t kb = smem_addr(sm + st * S::TILE_BYTES);
+    constexpr uint32_t kIdS = tc::idesc_bf16(kRowsTile, S::TOK, false, false);
+    constexpr uint32_t kIdO = tc::idesc_bf16(kRowsTile, D, false, true);
+    const uint32_t one = elect();
+    const auto scores = [&](int i) {
+      const int st = i % S::STAGES;
+      wait(&kfull[st], (i / S::STAGES) & 1);
+      tc::fence_after();
+      __syncwarp();
+      const uint32_t kb = smem_addr(sm + st * S::TILE_BYTES);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          tc::mma_bf16_ts(tmem + S::T_S + (i & 1) * S::TOK, tmem + S::T_Q + 8 * kk,
-                          tc::desc_kmajor(kb + (kk / 4) * (S::TOK * 128) + (kk % 4) * 32), kIdS,
-                          kk > 0);
+      for (int kk = 0; kk < D / 16; ++kk)
+        mma_elected(one, tmem + S::T_S + (i & 1) * S::TOK, tmem + S::T_Q + 8 * kk,
+                    tc::smem_desc(kb + (kk / 4) * 1024 + (kk % 4) * 32, 16, S::PAGE_BYTES / 2),
+                    kIdS, kk > 0);
+      if (one) {
         tc::commit(&sfull[i & 1]);
         tc::commit(&kfree[st]);
-        return true;
-      };
-      bool ok = mbar_wait_bounded(qfull, 0, a.status);
-      tc::fence_after();
-      ok = ok && scores(0);
-      for (int i = 0; ok && i < ntiles; ++i) {
-        if (i + 1 < ntiles) ok = scores(i + 1);
-        const int st = i % S::STAGES;
-        ok = ok && mbar_wait_bounded(&pfull[i & 1], (i >> 1) & 1, a.status) &&
-             mbar_wait_bounded(&vfull[st], (i / S::STAGES) & 1, a.status);
-        if (!ok) break;
-        tc::fence_after();
-        const uint32_t vb = smem_addr(sm + (S::STAGES + st) * S::TILE_BYTES);
-#pragma unroll
-        for (int kk = 0; kk < S::TOK / 16; ++kk)
-          tc::mma_bf16_ts(tmem, tmem + S::T_S + (i & 1) * S::TOK + 8 * kk,
-                          tc::desc_mnmajor(vb + kk * 2048, S::TOK * 128), kIdO, i > 0 || kk > 0);
-        tc::commit(&vfree[st]);
-        tc::commit(&ofull[i & 1]);
       }
+      __syncwarp();
+    };
+    wait(qfull, 0);
+    tc::fence_after();
+    scores(0);
+    for (int i = 0; i < ntiles; ++i) {
+      if (i + 1 < ntiles) scores(i + 1);
+      const int st = i % S::STAGES;
+      wait(&vfull[st], (i / S::STAGES) & 1);
+      wait(&pfull[i & 1], (i >> 1) & 1);
+      tc::fence_after();
+      __syncwarp();
+      const uint32_t vb = smem_addr(sm + (S::STAGES + st) * S::TILE_BYTES);
+#pragma unroll
+      for (int kk = 0; kk < S::PAGES; ++kk)
+        mma_elected(one, tmem, tmem + S::T_S + (i & 1) * S::TOK + 8 * kk,
+                    tc::smem_desc(vb + kk * S::PAGE_BYTES, 2048, 1024), kIdO, i > 0 || kk > 0);
+      if (one) {
+        tc::commit(&ofull[i & 1]);
+        tc::commit(&vfree[st]);
+      }
+      __syncwarp();
     }
+    ok = true;  // no product is in flight when TMEM goes back
+    wait(&ofull[(ntiles - 1) & 1], ((ntiles - 1) >> 1) & 1);
   } else {
     // ---------------------------------------------------------------- softmax
-    const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);  // this warp's TMEM lanes
-    const int member = tid / a.G, h = tid - member * a.G;
+    constexpr int kCols = S::TOK / 2;   // this thread's columns of a tile
+    constexpr int kOut = D / 2;         // and of O and Q
+    const int half = warp >> 2, r = tid & (kRowsTile - 1);
+    const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's TMEM lanes
+    const int member = r / a.G, h = r - member * a.G;
     const int b = member < tile.y ? a.members[tile.x + member] : -1;
     const bool live = b >= 0 && b < a.B;
+    const bool idle = !__any_sync(0xffffffffu, live);  // no row here: only the barriers
     const size_t out_row = live ? (size_t)b * a.Hq + kvh * a.G + h : 0;
-    // Tokens of this split that the row attends to (its context may end inside the prefix).
-    const int limit = live ? min(pages_of(b) - p0, npages) * kPageTok : 0;
+    // Pages of this split that the row attends to (its context may end inside the prefix).
+    const int limit = live ? min(pages_of(b) - p0, npages) : 0;
     // A negative scale turns q, so that the largest score stays the largest; a zero one
     // clears it.
     const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-    const uint32_t keep = a.scale_log2 == 0.f ? 0u : 0xffffffffu;
+    const uint32_t keep = a.scale_log2 == 0.f || !live ? 0u : 0xffffffffu;
     const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
     {
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + out_row * D);
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + out_row * D + half * kOut);
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = 0; c < kOut / 32; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const uint4 u = live ? src[4 * c + x] : make_uint4(0u, 0u, 0u, 0u);
+          const uint4 u = src[4 * c + x];
           w[4 * x] = u.x;
           w[4 * x + 1] = u.y;
           w[4 * x + 2] = u.z;
@@ -274,45 +358,56 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         }
 #pragma unroll
         for (int x = 0; x < 16; ++x) w[x] = (w[x] ^ flip) & keep;
-        tc::tmem_st16(mine + S::T_Q + 16 * c, w);
+        tc::tmem_st16(mine + S::T_Q + half * (kOut / 2) + 16 * c, w);
       }
       tc::tmem_wait_st();
       tc::fence_before();
       mbar_arrive(qfull);
     }
-    float m = -CUDART_INF_F, l = 0.f;  // reference maximum (log2 units) and sum
-    bool ok = true;
+    float m = -CUDART_INF_F, l = 0.f;  // reference maximum (log2 units), this half's sum
+    const auto grows = [&](float top) {
+      return top > m + kRescale || (m == -CUDART_INF_F && top > m);
+    };
     for (int i = 0; i < ntiles; ++i) {
-      ok = mbar_wait_bounded(&sfull[i & 1], (i >> 1) & 1, a.status);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (idle) {
+        if (soft_any(false)) soft_sync();
+        mbar_arrive(&pfull[i & 1]);
+        continue;
+      }
+      wait(&sfull[i & 1], (i >> 1) & 1);
       tc::fence_after();
       const uint32_t st = mine + S::T_S + (i & 1) * S::TOK;
-      float x[S::TOK];
+      float x[kCols];
 #pragma unroll
-      for (int c = 0; c < S::TOK / 32; ++c) tc::tmem_ld32(st + 32 * c, x + 32 * c);
-      const int left = limit - i * S::TOK;  // columns below it count
-      if (left < S::TOK)
+      for (int c = 0; c < kCols / 32; ++c) tc::tmem_ld32(st + half * kCols + 32 * c, x + 32 * c);
+      const int left = limit - i * S::PAGES - half * (S::PAGES / 2);  // pages that count
+      if (left < S::PAGES / 2)
 #pragma unroll
-        for (int c = 0; c < S::TOK; ++c) x[c] = c < left ? x[c] : -CUDART_INF_F;
+        for (int c = 0; c < kCols; ++c) x[c] = c / kPageTok < left ? x[c] : -CUDART_INF_F;
       float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-      for (int c = 0; c < S::TOK; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-      const bool grows = top > m + kRescale || (m == -CUDART_INF_F && top > m);
-      if (__any_sync(0xffffffffu, grows)) {
-        const float to = grows ? top : m;
+      for (int c = 0; c < kCols; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+      float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+      // Past this barrier both halves have read their scores (P goes over them).
+      tc::fence_before();
+      const bool any = soft_any(grows(top));
+      tc::fence_after();
+      if (any) {
+        s_half[half][r] = top;
+        soft_sync();
+        top = fmaxf(top, s_half[half ^ 1][r]);
+        const float to = grows(top) ? top : m;
         const float f = m == to ? 1.f : ex2(m - to);  // 0 from -inf
         if (i > 0) {
-          ok = mbar_wait_bounded(&ofull[(i - 1) & 1], ((i - 1) >> 1) & 1, a.status);
-          if (!__all_sync(0xffffffffu, ok)) break;
+          wait(&ofull[(i - 1) & 1], ((i - 1) >> 1) & 1);
           tc::fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = 0; c < kOut / 32; ++c) {
             float o[32];
-            tc::tmem_ld32(mine + 32 * c, o);
+            tc::tmem_ld32(mine + half * kOut + 32 * c, o);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] *= f;
-            tc::tmem_st32(mine + 32 * c, o);
+            tc::tmem_st32(mine + half * kOut + 32 * c, o);
           }
         }
         l *= f;
@@ -321,7 +416,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const float ref = m == -CUDART_INF_F ? 0.f : m;  // nothing seen yet: every p is 0
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < S::TOK / 32; ++c) {
+      for (int c = 0; c < kCols / 32; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -331,48 +426,322 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           sum[(2 * e + 1) & 3] += y1;
           w[e] = pack_bf16x2(y0, y1);
         }
-        tc::tmem_st16(st + 16 * c, w);
+        tc::tmem_st16(st + half * (kCols / 2) + 16 * c, w);
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tc::tmem_wait_st();
       tc::fence_before();
       mbar_arrive(&pfull[i & 1]);
     }
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
-      ok = mbar_wait_bounded(&ofull[(ntiles - 1) & 1], ((ntiles - 1) >> 1) & 1, a.status);
-      tc::fence_after();
-    }
-    if (__all_sync(0xffffffffu, ok)) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      const size_t part = out_row * a.num_splits + split;
+    wait(&ofull[(ntiles - 1) & 1], ((ntiles - 1) >> 1) & 1);
+    tc::fence_after();
+    soft_sync();  // s_half's last readers are done
+    s_half[half][r] = l;
+    soft_sync();
+    l += s_half[half ^ 1][r];
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const size_t part = out_row * a.num_splits + split;
+    // Each thread stages its half row in the stages, which no copy or product uses any
+    // more, and sends it off as bulk copies: a row is contiguous in global memory.
+    uint8_t* stage = sm + tid * S::PITCH;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        float o[32];
-        tc::tmem_ld32(mine + 32 * c, o);
-        if (live) {
-          float4* dst = reinterpret_cast<float4*>(a.part_out + part * D + 32 * c);
+    for (int c = 0; c < kOut; c += S::PIECE) {
+      if (c > 0) bulk_wait_read_all();
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[e] = make_float4(o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv,
-                                 o[4 * e + 3] * inv);
-        }
+      for (int p = 0; p < S::PIECE / 32; ++p) {
+        float o[32];
+        tc::tmem_ld32(mine + half * kOut + c + 32 * p, o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          reinterpret_cast<float4*>(stage + 128 * p)[e] = make_float4(
+              o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv);
       }
-      if (live)
-        a.part_lse[part] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f
-                                   : (l == 0.f ? -CUDART_INF_F : l);  // a NaN stays one
+      fence_proxy_async_smem();
+      if (live && ok) {
+        bulk_s2g(a.part_out + part * D + half * kOut + c, stage, S::PIECE * 4);
+        bulk_commit();
+      }
     }
+    if (live && half == 0)
+      a.part_lse[part] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f
+                                 : (l == 0.f ? -CUDART_INF_F : l);  // a NaN stays one
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the parts are written
   }
   __syncwarp();
   tc::fence_before();
   __syncthreads();
-  if (warp == 5) tc::tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+}
+
+// ---------------------------------------------------------------- the sequences' own pages
+constexpr int kTailWarps = 2;
+constexpr int kTailStages = 3;
+constexpr int kTailHeads = 8;        // query heads of a unit
+constexpr int kTailMaxPages = 32;    // pages of a unit: a lane holds the id of one
+constexpr int kSlabRows = 1024;      // rows a warp searches for its unit
+
+struct TailArgs {
+  const uint16_t *q, *kv_pool;
+  const int32_t *block_table, *ctx_len, *first_page;
+  float *part_out, *part_lse;
+  int* counters;
+  long long num_pages;
+  float scale_log2;
+  int B, Hq, Hkv, G, HG, max_pages, pages_per_split, num_splits;
+  unsigned int* status;
+};
+
+// A row's own pages, [skip, skip + pages) of its block table, and the tokens they hold.
+struct OwnPages {
+  int skip, pages, tokens;
+};
+__device__ __forceinline__ OwnPages own_pages(int ctx, int first_page, int max_pages) {
+  OwnPages o;
+  ctx = (int)max(0ll, min((long long)ctx, (long long)max_pages * kPageTok));
+  // A page that the context ends in is never left to the prefix.
+  o.skip = min(max(0, min(first_page, max_pages)), ctx / kPageTok);
+  o.tokens = ctx - o.skip * kPageTok;
+  o.pages = (o.tokens + kPageTok - 1) / kPageTok;
+  return o;
+}
+
+template <int D>
+__global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
+  constexpr int ROW = D * 2, KV = kPageTok * ROW, STAGE = 2 * KV, KSTEPS = D / 16;
+  constexpr unsigned kAll = 0xffffffffu;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* stage = smem + warp * kTailStages * STAGE;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kTailWarps * kTailStages * STAGE) +
+                  warp * kTailStages;
+  pdl_trigger();
+  if (lane == 0) {
+    for (int i = 0; i < kTailStages; ++i) mbar_init(&bar[i], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  const int slab = blockIdx.y, row0 = slab * kSlabRows;
+  const int rows = min(kSlabRows, a.B - row0);
+  const int groups = a.Hkv * a.HG;
+
+  struct Unit {
+    int b, kvh, head0, heads, split, n, tokens;  // n pages; tokens of them count
+    int page;                                    // lane i: the id of page i
+  };
+  const auto take = [&]() {
+    int t = 0;
+    if (lane == 0) t = atomicAdd(a.counters + slab, 1);
+    return t;
+  };
+  // Unit t of the slab: chunk t / groups of the rows' chunks laid end to end. Uniform over
+  // the warp; u.n == 0 past the last one.
+  const auto resolve = [&](int t) {
+    Unit u;
+    t = __shfl_sync(kAll, t, 0);
+    const int want = t / groups, hg = t - want * groups;
+    u.n = 0;
+    int before = 0;
+    for (int r = 0; r < rows; r += 32) {
+      OwnPages o{0, 0, 0};
+      if (r + lane < rows)
+        o = own_pages(a.ctx_len[row0 + r + lane], a.first_page[row0 + r + lane], a.max_pages);
+      const int mine = min((o.pages + a.pages_per_split - 1) / a.pages_per_split, a.num_splits);
+      int incl = mine;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(kAll, incl, off);
+        if (lane >= off) incl += y;
+      }
+      const unsigned hit = __ballot_sync(kAll, want < before + incl);
+      if (hit != 0u) {
+        const int src = __ffs(hit) - 1;
+        const int chunk = want - before - (__shfl_sync(kAll, incl, src) - __shfl_sync(kAll, mine, src));
+        const int skip = __shfl_sync(kAll, o.skip, src), pages = __shfl_sync(kAll, o.pages, src);
+        const int tokens = __shfl_sync(kAll, o.tokens, src);
+        u.b = row0 + r + src;
+        u.split = chunk;
+        u.n = min(a.pages_per_split, pages - chunk * a.pages_per_split);
+        u.tokens = min(u.n * kPageTok, tokens - chunk * a.pages_per_split * kPageTok);
+        u.page = lane < u.n ? a.block_table[(size_t)u.b * a.max_pages + skip +
+                                            chunk * a.pages_per_split + lane]
+                            : 0;
+        u.kvh = hg / a.HG;
+        u.head0 = u.kvh * a.G + (hg - u.kvh * a.HG) * kTailHeads;
+        u.heads = min(kTailHeads, (u.kvh + 1) * a.G - u.head0);
+        return u;
+      }
+      before += __shfl_sync(kAll, incl, 31);
+    }
+    return u;
+  };
+  int issued = 0, consumed = 0;  // pages of all units, in order through the stages
+  const auto issue = [&](const Unit& u, int i) {
+    int page = __shfl_sync(kAll, u.page, i);
+    if (lane == 0) {
+      if (page < 0 || page >= a.num_pages) {
+        flag_device(a.status, DEV_BAD_INDEX);
+        page = 0;  // keep the copy in bounds; the status word reports the fault
+      }
+      const int s = issued % kTailStages;
+      mbar_arrive_expect_tx(&bar[s], STAGE);
+      bulk_g2s(stage + s * STAGE,
+               reinterpret_cast<const uint8_t*>(a.kv_pool) + ((size_t)page * a.Hkv + u.kvh) * STAGE,
+               STAGE, &bar[s]);
+    }
+    ++issued;
+  };
+  const int mi = lane >> 3, r8 = lane & 7;
+  const int tk = r8 + 8 * (mi & 1);   // token row this lane addresses for K
+  const int tv = r8 + 8 * (mi >> 1);  // token row this lane addresses for V^T
+  // After a bounded wait has given up on this device, later CTAs take no work.
+  bool ok = a.status == nullptr ||
+            !(*reinterpret_cast<volatile unsigned int*>(a.status) & DEV_WAIT_TIMEOUT);
+  ok = __all_sync(kAll, ok);
+  Unit cur;
+  cur.n = 0;
+  if (ok) cur = resolve(take());
+  int cur_issued = 0;
+  while (ok && cur.n > 0) {
+    while (issued - consumed < kTailStages && cur_issued < cur.n) issue(cur, cur_issued++);
+    const int t_next = take();
+    Unit nxt;
+    nxt.n = 0;
+    int nxt_issued = 0;
+    bool have_next = false;
+    // Q^T as the B operand: b0 = q[n][16kk + 2c .. +1], b1 = q[n][16kk + 8 + 2c .. +1].
+    uint32_t qf[KSTEPS][2];
+    {
+      const int n = lane >> 2, c = lane & 3;
+      const bool valid = n < cur.heads;
+      const uint16_t* qp = a.q + ((size_t)cur.b * a.Hq + cur.head0 + (valid ? n : 0)) * D;
+#pragma unroll
+      for (int kk = 0; kk < KSTEPS; ++kk) {
+        qf[kk][0] = valid ? *reinterpret_cast<const uint32_t*>(qp + 16 * kk + 2 * c) : 0u;
+        qf[kk][1] = valid ? *reinterpret_cast<const uint32_t*>(qp + 16 * kk + 8 + 2 * c) : 0u;
+      }
+    }
+    float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F;  // running max of heads 2c, 2c+1 (log2 units)
+    float l0 = 0.f, l1 = 0.f;                      // this lane's partial sums
+    float o[KSTEPS][4];
+#pragma unroll
+    for (int mt = 0; mt < KSTEPS; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
+    for (int j = 0; j < cur.n; ++j) {
+      if (cur_issued == cur.n && !have_next) {
+        nxt = resolve(t_next);
+        have_next = true;
+        while (issued - consumed < kTailStages && nxt_issued < nxt.n) issue(nxt, nxt_issued++);
+      }
+      const int s = consumed % kTailStages;
+      ok = mbar_wait_bounded(&bar[s], (consumed / kTailStages) & 1, a.status);
+      ok = __all_sync(kAll, ok);
+      if (!ok) break;
+      const uint32_t kbase = smem_addr(stage + s * STAGE), vbase = kbase + KV;
+      const int left = cur.tokens - j * kPageTok;  // tokens of the page that count
+      if (left < kPageTok) {
+        // Rows past the context hold whatever the pool held (possibly Inf/NaN bits); their
+        // probability is 0, but 0 * Inf would poison the sum.
+        uint4* vrows = reinterpret_cast<uint4*>(stage + s * STAGE + KV);
+        for (int c = left * (ROW / 16) + lane; c < kPageTok * (ROW / 16); c += 32)
+          vrows[c] = make_uint4(0u, 0u, 0u, 0u);
+        __syncwarp();
+      }
+      float sa[2][4];  // two accumulators halve the dependent chain of the scores
+#pragma unroll
+      for (int x = 0; x < 2; ++x) sa[x][0] = sa[x][1] = sa[x][2] = sa[x][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KSTEPS; ++kk) {
+        const int chunk = 2 * kk + (mi >> 1);
+        uint32_t a0, a1, a2, a3;
+        ldsm_x4(kbase + tk * ROW + ((chunk ^ (tk & 7)) << 4), a0, a1, a2, a3);
+        mma_bf16_16816(sa[kk & 1], a0, a1, a2, a3, qf[kk][0], qf[kk][1]);
+      }
+      const int tok = lane >> 2;
+      const bool lo = tok < left, hi = tok + 8 < left;
+      const float x0 = lo ? (sa[0][0] + sa[1][0]) * a.scale_log2 : -CUDART_INF_F;
+      const float x1 = lo ? (sa[0][1] + sa[1][1]) * a.scale_log2 : -CUDART_INF_F;
+      const float x2 = hi ? (sa[0][2] + sa[1][2]) * a.scale_log2 : -CUDART_INF_F;
+      const float x3 = hi ? (sa[0][3] + sa[1][3]) * a.scale_log2 : -CUDART_INF_F;
+      float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
+#pragma unroll
+      for (int off = 4; off <= 16; off <<= 1) {
+        t0 = fmaxf(t0, __shfl_xor_sync(kAll, t0, off));
+        t1 = fmaxf(t1, __shfl_xor_sync(kAll, t1, off));
+      }
+      // The first token of every page counts, so t0 / t1 are finite for finite scores.
+      const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+      const float c0 = exp2f(m0 - n0), c1 = exp2f(m1 - n1);
+      const float p0 = exp2f(x0 - n0), p1 = exp2f(x1 - n1);
+      const float p2 = exp2f(x2 - n0), p3 = exp2f(x3 - n1);
+      l0 = fmaf(l0, c0, p0 + p2);
+      l1 = fmaf(l1, c1, p1 + p3);
+      m0 = n0;
+      m1 = n1;
+      const uint32_t pb0 = movmatrix_t(pack_bf16x2(p0, p1));
+      const uint32_t pb1 = movmatrix_t(pack_bf16x2(p2, p3));
+#pragma unroll
+      for (int mt = 0; mt < KSTEPS; ++mt) {
+        o[mt][0] *= c0;
+        o[mt][1] *= c1;
+        o[mt][2] *= c0;
+        o[mt][3] *= c1;
+        const int chunk = 2 * mt + (mi & 1);
+        uint32_t a0, a1, a2, a3;
+        ldsm_x4_t(vbase + tv * ROW + ((chunk ^ (tv & 7)) << 4), a0, a1, a2, a3);
+        mma_bf16_16816(o[mt], a0, a1, a2, a3, pb0, pb1);
+      }
+      ++consumed;
+      __syncwarp();
+      if (cur_issued < cur.n || (have_next && nxt_issued < nxt.n)) {
+        if (lane == 0) fence_proxy_async_smem();
+        if (cur_issued < cur.n)
+          issue(cur, cur_issued++);
+        else
+          issue(nxt, nxt_issued++);
+      }
+    }
+    if (!ok) break;
+#pragma unroll
+    for (int off = 4; off <= 16; off <<= 1) {
+      l0 += __shfl_xor_sync(kAll, l0, off);
+      l1 += __shfl_xor_sync(kAll, l1, off);
+    }
+    // O^T: this lane holds dims d0 + 16 mt (+ 8) of heads h0, h0 + 1.
+    const int d0 = lane >> 2, h0 = 2 * (lane & 3);
+    const float i0 = 1.f / l0, i1 = 1.f / l1;
+    const size_t part = ((size_t)cur.b * a.Hq + cur.head0 + h0) * a.num_splits + cur.split;
+    float* w0 = a.part_out + part * D + d0;
+    float* w1 = w0 + (size_t)a.num_splits * D;
+    if (h0 < cur.heads) {
+#pragma unroll
+      for (int mt = 0; mt < KSTEPS; ++mt) {
+        w0[16 * mt] = o[mt][0] * i0;
+        w0[16 * mt + 8] = o[mt][2] * i0;
+      }
+      if (d0 == 0) a.part_lse[part] = (m0 + log2f(l0)) * 0.6931471805599453f;
+    }
+    if (h0 + 1 < cur.heads) {
+#pragma unroll
+      for (int mt = 0; mt < KSTEPS; ++mt) {
+        w1[16 * mt] = o[mt][1] * i1;
+        w1[16 * mt + 8] = o[mt][3] * i1;
+      }
+      if (d0 == 0) a.part_lse[part + a.num_splits] = (m1 + log2f(l1)) * 0.6931471805599453f;
+    }
+    cur = nxt;
+    cur_issued = nxt_issued;
+  }
+  // A wait gave up (already flagged): the copies in flight land before the CTA ends.
+  for (; consumed < issued; ++consumed)
+    if (!mbar_wait_bounded(&bar[consumed % kTailStages], (consumed / kTailStages) & 1, a.status)) break;
+  // The grid ends after the prefix kernel's, so that what waits for this one waits for
+  // both. One CTA sees to that; the others leave their SMs.
+  if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
 }
 
 // The parts of each (sequence, head) row: those of its prefix, then its own tail's.
-// D / 4 threads hold a float4 of the row each, the CTA's other threads take other parts;
-// the weights e^(lse - M) are made once in shared memory.
-constexpr int kMergeThreads2 = 256;
+// kWarps warps share a row (a warp's lane holds D / 32 of its columns) and take its
+// parts in turn; a warp holds the parts' weights e^(lse - M), 32 at a time, in its lanes.
+constexpr int kMergeThreads = 256;
 constexpr int kMergeMax = 1024;  // parts of one row
 
 struct MergeArgs {
@@ -380,76 +749,104 @@ struct MergeArgs {
   const int32_t *ctx_len, *first_page;
   uint16_t* out;
   float* lse_out;
-  int Hq, max_pages, pre_pps, pre_splits, tail_pps, tail_splits;
+  int rows, Hq, max_pages, pre_pps, pre_splits, tail_pps, tail_splits;
+  unsigned int* status;
 };
 
-template <int D>
-__global__ void __launch_bounds__(kMergeThreads2) merge_parts_kernel(const MergeArgs a) {
-  constexpr int kCols = D / 4, kLanes = kMergeThreads2 / kCols;
-  __shared__ float w[kMergeMax];
-  __shared__ float red[kMergeThreads2 / 32], sums[kLanes];
-  __shared__ float4 acc_s[kMergeThreads2];
+template <int D, int kWarps>
+__global__ void __launch_bounds__(kMergeThreads) merge_parts_kernel(const MergeArgs a) {
+  constexpr int kPer = D / 32;                       // columns of a lane
+  constexpr int kRows = kMergeThreads / 32 / kWarps; // rows of the CTA
+  constexpr unsigned kAll = 0xffffffffu;
+  __shared__ float acc_s[kMergeThreads / 32][kWarps > 1 ? D : 1];
+  __shared__ float sum_s[kMergeThreads / 32];
   pdl_wait();
   pdl_trigger();
-  const size_t row = blockIdx.x;
-  const int b = (int)(row / a.Hq), tid = threadIdx.x;
-  const int ctx = max(a.ctx_len[b], 0);
-  const int skip = min(max(0, min(a.first_page[b], a.max_pages)), ctx / kPageTok);
-  const int pages = min((ctx - skip * kPageTok + kPageTok - 1) / kPageTok, a.max_pages - skip);
-  const int n_pre = min((skip + a.pre_pps - 1) / a.pre_pps, a.pre_splits);
-  const int n = n_pre + min((pages + a.tail_pps - 1) / a.tail_pps, a.tail_splits);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp % kWarps;
+  const int row = blockIdx.x * kRows + warp / kWarps;
+  const bool live = row < a.rows;
+  const int b = live ? row / a.Hq : 0;
+  const int ctx = live ? a.ctx_len[b] : 0, first_page = live ? a.first_page[b] : 0;
+  const OwnPages own_pg = own_pages(ctx, first_page, a.max_pages);
+  const int need_pre = (own_pg.skip + a.pre_pps - 1) / a.pre_pps;
+  const int need_own = (own_pg.pages + a.tail_pps - 1) / a.tail_pps;
+  const int n_pre = min(need_pre, a.pre_splits);
+  const int n = n_pre + min(need_own, a.tail_splits);
+  // A context outside the block table, or more pages than the splits cover: clamped.
+  if (lane == 0 && (ctx < 0 || (long long)ctx > (long long)a.max_pages * kPageTok ||
+                    first_page < 0 || first_page > a.max_pages || need_pre > n_pre ||
+                    need_own > n - n_pre))
+    flag_device(a.status, DEV_BAD_INDEX);
+  const size_t pre = (size_t)row * a.pre_splits, own = (size_t)row * a.tail_splits;
   const auto lse_at = [&](int s) {
-    return s < n_pre ? a.pre_lse[row * a.pre_splits + s] : a.tail_lse[row * a.tail_splits + s - n_pre];
+    return s < n_pre ? a.pre_lse[pre + s] : a.tail_lse[own + s - n_pre];
   };
-  float m = -CUDART_INF_F;
-  for (int s = tid; s < n; s += kMergeThreads2) {
-    w[s] = lse_at(s);
-    m = fmaxf(m, w[s]);
-  }
+  // The first 32 parts' lse stay in the lanes; more (many splits) are read again below.
+  const float first = lane < n ? lse_at(lane) : -CUDART_INF_F;
+  float m = first;
+  for (int s = lane + 32; s < n; s += 32) m = fmaxf(m, lse_at(s));
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  if ((tid & 31) == 0) red[tid >> 5] = m;
-  __syncthreads();
+  for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, off));
+  float acc[kPer], sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kMergeThreads2 / 32; ++i) m = fmaxf(m, red[i]);
-  __syncthreads();
-  const int col = tid % kCols, first = tid / kCols;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-  for (int s = first; s < n; s += kLanes) {
-    const float ls = w[s];
-    if (ls == -CUDART_INF_F) continue;  // an empty part
-    const float e = __expf(ls - m);
-    const float* o = s < n_pre ? a.pre_out + (row * a.pre_splits + s) * D
-                               : a.tail_out + (row * a.tail_splits + s - n_pre) * D;
-    const float4 v = reinterpret_cast<const float4*>(o)[col];
-    acc.x = fmaf(e, v.x, acc.x);
-    acc.y = fmaf(e, v.y, acc.y);
-    acc.z = fmaf(e, v.z, acc.z);
-    acc.w = fmaf(e, v.w, acc.w);
-    sum += e;
-  }
-  acc_s[tid] = acc;
-  if (col == 0) sums[first] = sum;
-  __syncthreads();
-  if (tid < kCols) {
-    float total = 0.f;
-    for (int i = 0; i < kLanes; ++i) total += sums[i];
-    for (int i = 1; i < kLanes; ++i) {
-      const float4 v = acc_s[i * kCols + tid];
-      acc.x += v.x;
-      acc.y += v.y;
-      acc.z += v.z;
-      acc.w += v.w;
+  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    const float ls = s0 == 0 ? first : (s0 + lane < n ? lse_at(s0 + lane) : -CUDART_INF_F);
+    const float e = ls == -CUDART_INF_F ? 0.f : __expf(ls - m);
+    const int cnt = min(32, n - s0);
+#pragma unroll 4
+    for (int s = w; s < cnt; s += kWarps) {
+      const float es = __shfl_sync(kAll, e, s);
+      const float* o = s0 + s < n_pre ? a.pre_out + (pre + s0 + s) * D
+                                      : a.tail_out + (own + s0 + s - n_pre) * D;
+      float v[kPer];
+      if constexpr (kPer == 2) {
+        const float2 u = reinterpret_cast<const float2*>(o)[lane];
+        v[0] = u.x;
+        v[1] = u.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer / 4; ++i) {
+          const float4 u = reinterpret_cast<const float4*>(o)[lane + 32 * i];
+          v[4 * i] = u.x;
+          v[4 * i + 1] = u.y;
+          v[4 * i + 2] = u.z;
+          v[4 * i + 3] = u.w;
+        }
+      }
+      sum += es;
+      if (es != 0.f)  // an empty part holds nothing (a NaN weight passes)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) acc[i] = fmaf(es, v[i], acc[i]);
     }
-    const float inv = n == 0 || total == 0.f ? 0.f : 1.f / total;
-    uint2 u;
-    u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-    u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-    reinterpret_cast<uint2*>(a.out + row * D)[tid] = u;
-    if (tid == 0 && a.lse_out != nullptr)
-      a.lse_out[row] = total == 0.f ? -CUDART_INF_F : m + logf(total);
   }
+  if constexpr (kWarps > 1) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc_s[warp][i * 32 + lane] = acc[i];
+    if (lane == 0) sum_s[warp] = sum;
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int o = 1; o < kWarps; ++o) {
+      sum += sum_s[warp + o];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) acc[i] += acc_s[warp + o][i * 32 + lane];
+    }
+  }
+  if (!live) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* out = a.out + (size_t)row * D;
+  if constexpr (kPer == 2) {
+    reinterpret_cast<uint32_t*>(out)[lane] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer / 4; ++i)
+      reinterpret_cast<uint2*>(out)[lane + 32 * i] =
+          make_uint2(pack_bf16x2(acc[4 * i] * inv, acc[4 * i + 1] * inv),
+                     pack_bf16x2(acc[4 * i + 2] * inv, acc[4 * i + 3] * inv));
+  }
+  if (lane == 0 && a.lse_out != nullptr)
+    a.lse_out[row] = sum == 0.f ? -CUDART_INF_F : m + logf(sum);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -466,15 +863,15 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// The pool as [block = (page, head, K|V)][64-column slice][token][64]: one box is the 16
-// tokens of one slice, x always 0.
-int encode_pool(CUtensorMap* map, const void* pool, int D, long long blocks) {
+// The pool as [block = (page, head, K|V)][64-column slice][token][64]: a box is `tokens`
+// (8 or 16) tokens of a block, x always 0.
+int encode_pool(CUtensorMap* map, const void* pool, int D, long long blocks, int tokens) {
   auto fn = encode_fn();
   if (fn == nullptr)
     return set_error(SC_ERR_CUDA, "sc_shared_prefix_attention: cuTensorMapEncodeTiled unavailable");
   cuuint64_t dims[4] = {64, kPageTok, (cuuint64_t)D / 64, (cuuint64_t)blocks};
   cuuint64_t strides[3] = {(cuuint64_t)D * 2, 128, (cuuint64_t)kPageTok * D * 2};
-  cuuint32_t box[4] = {64, kPageTok, 1, 1};
+  cuuint32_t box[4] = {64, (cuuint32_t)tokens, (cuuint32_t)D / 64, 1};
   cuuint32_t step[4] = {1, 1, 1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pool), dims,
                         strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -486,30 +883,47 @@ int encode_pool(CUtensorMap* map, const void* pool, int D, long long blocks) {
 }
 
 template <int D>
-int launch_shared(const CUtensorMap& map, const PrefixArgs& p, const MergeArgs& m, int ntiles,
-                  const sc_bf16* kv_pool, const int32_t* seq_order, float scale,
-                  float* tail_out, float* tail_lse, cudaStream_t s) {
+int launch_shared(const CUtensorMap* maps, const PrefixArgs& p, const MergeArgs& m, int ntiles,
+                  const TailArgs& t, cudaStream_t s) {
   const char* name = "sc_shared_prefix_attention";
   using S = PrefixShape<D>;
+  constexpr size_t tail_smem =
+      (size_t)kTailWarps * kTailStages * (2 * S::PAGE_BYTES + sizeof(uint64_t));
   static int configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    const cudaError_t err = cudaFuncSetAttribute(
+    cudaError_t err = cudaFuncSetAttribute(
         prefix_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    // All of the SM's memory as shared memory: a tail CTA goes beside this one.
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(prefix_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 cudaSharedmemCarveoutMaxShared);
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(tail_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)tail_smem);
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(tail_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 cudaSharedmemCarveoutMaxShared);
     if (err != cudaSuccess)
       return set_error(SC_ERR_CUDA, "%s: smem attribute: %s", name, cudaGetErrorString(err));
     configured[dev] = 1;
   }
   cudaError_t err = launch_pdl(prefix_kernel<D>, dim3(p.num_splits, p.Hkv, ntiles),
-                               dim3(kPrefixThreads), S::SMEM, s, map, p);
+                               dim3(kPrefixThreads), S::SMEM, s, maps[0], maps[1], p);
   if (err != cudaSuccess)
     return set_error(SC_ERR_CUDA, "%s: launch: %s", name, cudaGetErrorString(err));
-  if (int rc = launch_decode_tail(p.q, kv_pool, p.num_pages, p.block_table, p.ctx_len, seq_order,
-                                  m.first_page, p.B, p.Hq, p.Hkv, D, p.max_pages, m.tail_pps,
-                                  m.tail_splits, scale, tail_out, tail_lse, s))
-    return rc;
-  err = launch_pdl(merge_parts_kernel<D>, dim3(p.B * p.Hq), dim3(kMergeThreads2), 0, s, m);
+  // Two CTAs an SM (one while a prefix CTA is there), fewer where there is less work.
+  const long long units = (long long)std::min(p.B, kSlabRows) * t.Hkv * t.HG * t.num_splits;
+  const int ctas = (int)std::min(2ll * 148, (units + kTailWarps - 1) / kTailWarps);
+  err = launch_pdl(tail_kernel<D>, dim3(ctas, p.slabs), dim3(kTailWarps * 32), tail_smem, s, t);
+  if (err != cudaSuccess)
+    return set_error(SC_ERR_CUDA, "%s: launch: %s", name, cudaGetErrorString(err));
+  // A warp a row while the rows fill the GPU; few rows of many parts get eight.
+  const bool wide = m.rows * 8 <= 148 * 64 && m.pre_splits + m.tail_splits > 4;
+  const int per_cta = wide ? 1 : kMergeThreads / 32;
+  err = launch_pdl(wide ? merge_parts_kernel<D, 8> : merge_parts_kernel<D, 1>,
+                   dim3((m.rows + per_cta - 1) / per_cta), dim3(kMergeThreads), 0, s, m);
   if (err != cudaSuccess)
     return set_error(SC_ERR_CUDA, "%s: launch: %s", name, cudaGetErrorString(err));
   return check_launch(name);
@@ -520,11 +934,11 @@ int launch_shared(const CUtensorMap& map, const PrefixArgs& p, const MergeArgs& 
 
 extern "C" int sc_shared_prefix_attention(
     const sc_bf16* q, const sc_bf16* kv_pool, int64_t num_pages, const int32_t* block_table,
-    const int32_t* ctx_len, const int32_t* seq_order, const int32_t* prefix_pages,
+    const int32_t* ctx_len, const int32_t* prefix_pages,
     const int32_t* tiles, const int32_t* members, int ntiles, int B, int Hq, int Hkv, int D, int P,
     int max_pages, int prefix_pages_per_split, int prefix_splits, int pages_per_split,
     int num_splits, float scale, float* prefix_out, float* prefix_lse, float* part_out,
-    float* part_lse, sc_bf16* out, float* lse_out, void* stream) {
+    float* part_lse, int32_t* counters, sc_bf16* out, float* lse_out, void* stream) {
   const char* name = "sc_shared_prefix_attention";
   SC_REQUIRE(B >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0, SC_ERR_INVALID,
              "%s: bad heads Hq=%d Hkv=%d", name, Hq, Hkv);
@@ -535,7 +949,7 @@ extern "C" int sc_shared_prefix_attention(
              Hq / Hkv);
   if (B == 0) return SC_OK;
   SC_REQUIRE(q && kv_pool && block_table && ctx_len && prefix_pages && tiles && members && out &&
-                 prefix_out && prefix_lse && part_out && part_lse,
+                 prefix_out && prefix_lse && part_out && part_lse && counters,
              SC_ERR_INVALID, "%s: null pointer", name);
   SC_REQUIRE(num_pages > 0 && max_pages > 0 && ntiles > 0 && prefix_pages_per_split > 0 &&
                  prefix_splits > 0 && pages_per_split > 0 && num_splits > 0,
@@ -543,15 +957,18 @@ extern "C" int sc_shared_prefix_attention(
              max_pages, ntiles, prefix_splits, prefix_pages_per_split, num_splits, pages_per_split);
   SC_REQUIRE(prefix_splits + num_splits <= sc::kMergeMax, SC_ERR_INVALID,
              "%s: %d + %d splits, at most %d", name, prefix_splits, num_splits, sc::kMergeMax);
-  SC_REQUIRE(B <= 65535 && ntiles <= 65535 && Hkv * ((Hq / Hkv + 7) / 8) <= 65535 &&
+  SC_REQUIRE(B <= 65535 && ntiles <= 65535 && Hkv <= 65535 && Hkv * ((Hq / Hkv + 7) / 8) <= 65535 &&
                  num_pages * Hkv * 2 < (1ll << 31),
              SC_ERR_INVALID, "%s: grid or pool too large", name);
+  SC_REQUIRE(pages_per_split <= sc::kTailMaxPages, SC_ERR_UNSUPPORTED,
+             "%s: %d pages per split, at most %d", name, pages_per_split, sc::kTailMaxPages);
   const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   SC_REQUIRE(aligned(q) && aligned(kv_pool) && aligned(out) && aligned(prefix_out) &&
                  aligned(part_out) && aligned(tiles),
              SC_ERR_INVALID, "%s: operands must be 16-byte aligned", name);
-  CUtensorMap map;
-  if (int rc = sc::encode_pool(&map, kv_pool, D, num_pages * Hkv * 2)) return rc;
+  CUtensorMap maps[2];  // half pages (K), pages (V)
+  for (int i = 0; i < 2; ++i)
+    if (int rc = sc::encode_pool(&maps[i], kv_pool, D, num_pages * Hkv * 2, 8 * (i + 1))) return rc;
   sc::PrefixArgs p;
   p.q = q;
   p.block_table = block_table;
@@ -560,6 +977,8 @@ extern "C" int sc_shared_prefix_attention(
   p.members = members;
   p.part_out = prefix_out;
   p.part_lse = prefix_lse;
+  p.counters = counters;
+  p.slabs = (B + sc::kSlabRows - 1) / sc::kSlabRows;
   p.num_pages = num_pages;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.B = B;
@@ -579,15 +998,37 @@ extern "C" int sc_shared_prefix_attention(
   m.first_page = prefix_pages;
   m.out = out;
   m.lse_out = lse_out;
+  m.rows = B * Hq;
   m.Hq = Hq;
   m.max_pages = max_pages;
   m.pre_pps = prefix_pages_per_split;
   m.pre_splits = prefix_splits;
   m.tail_pps = pages_per_split;
   m.tail_splits = num_splits;
+  m.status = p.status;
+  sc::TailArgs t;
+  t.q = q;
+  t.kv_pool = kv_pool;
+  t.block_table = block_table;
+  t.ctx_len = ctx_len;
+  t.first_page = prefix_pages;
+  t.part_out = part_out;
+  t.part_lse = part_lse;
+  t.counters = counters;
+  t.num_pages = num_pages;
+  t.scale_log2 = p.scale_log2;
+  t.B = B;
+  t.Hq = Hq;
+  t.Hkv = Hkv;
+  t.G = p.G;
+  t.HG = (p.G + sc::kTailHeads - 1) / sc::kTailHeads;
+  t.max_pages = max_pages;
+  t.pages_per_split = pages_per_split;
+  t.num_splits = num_splits;
+  t.status = p.status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const auto launch = D == 64    ? sc::launch_shared<64>
                       : D == 128 ? sc::launch_shared<128>
                                  : sc::launch_shared<256>;
-  return launch(map, p, m, ntiles, kv_pool, seq_order, scale, part_out, part_lse, s);
+  return launch(maps, p, m, ntiles, t, s);
 }

@@ -421,7 +421,8 @@ class PrefixGroups:
     """
 
     def __init__(self, groups, batch: int, q_heads: int, kv_heads: int, head_dim: int,
-                 device: str | torch.device = "cuda", sms: int | None = None):
+                 device: str | torch.device = "cuda", sms: int | None = None,
+                 pages_per_split: int | None = None):
         if q_heads % kv_heads or q_heads // kv_heads > PREFIX_ROWS:
             raise ValueError(f"PrefixGroups: {q_heads} query heads over {kv_heads} kv heads")
         if head_dim not in (64, 128, 256):
@@ -450,7 +451,7 @@ class PrefixGroups:
         self.max_prefix_pages = max((t[2] for t in tiles), default=0)
         self.min_first_page = min(first_page, default=0)
         self.pages_per_split, self.num_splits = prefix_split_plan(
-            [t[2] for t in tiles], kv_heads, head_dim, sms or sm_count(device))
+            [t[2] for t in tiles], kv_heads, head_dim, sms or sm_count(device), pages_per_split)
         # One transfer: tiles [ntiles, 4], then first_page [batch], then members.
         flat = torch.tensor([x for t in tiles for x in t] + first_page + members,
                             dtype=torch.int32).to(device)
@@ -459,13 +460,34 @@ class PrefixGroups:
         self.members = flat[4 * len(tiles) + batch:]
 
 
-def prefix_split_plan(tile_pages: list, kv_heads: int, head_dim: int, sms: int) -> tuple:
-    """(pages_per_split, num_splits) of the shared pages: about one CTA per SM over all
-    tiles and kv heads, in whole tiles of the kernel (4 pages at D = 256, else 8)."""
+def prefix_split_plan(tile_pages: list, kv_heads: int, head_dim: int, sms: int,
+                      pages_per_split: int | None = None) -> tuple:
+    """(pages_per_split, num_splits) of the shared pages, in whole tiles of the kernel (4
+    pages at D = 256, else 8): as many equal splits as give at most one CTA per SM over
+    all tiles and kv heads."""
     unit = 4 if head_dim == 256 else 8
-    work = sum(tile_pages) * kv_heads
-    pps = max(unit, -(-work // (sms * unit)) * unit)
-    return pps, max(1, -(-max(tile_pages, default=1) // pps))
+    longest = max(tile_pages, default=1)
+    if not pages_per_split:
+        work = sum(tile_pages) * kv_heads  # pages of all (tile, kv head)s
+        pages_per_split = max(2 * unit, -(-work // sms))
+        ctas = lambda p: sum(-(-t // p) for t in tile_pages) * kv_heads  # noqa: E731
+        while ctas(pages_per_split) > sms and pages_per_split < longest:
+            pages_per_split += unit
+    pps = -(-pages_per_split // unit) * unit
+    return pps, max(1, -(-longest // pps))
+
+
+def tail_split_plan(batch: int, q_heads: int, kv_heads: int, max_pages: int,
+                    pages_per_split: int | None, total_pages: int | None, sms: int) -> tuple:
+    """(pages_per_split, num_splits) of the sequences' own pages beside a prefix: units of
+    work of up to 32 pages, small enough that every warp of two CTAs an SM gets some."""
+    if not pages_per_split:
+        groups = kv_heads * ((q_heads // kv_heads + 7) // 8)
+        work = (total_pages or batch * max_pages) * groups
+        pages_per_split = 4
+        while pages_per_split < 16 and work / (2 * pages_per_split) >= 4 * sms:
+            pages_per_split *= 2
+    return pages_per_split, max(1, -(-max_pages // pages_per_split))
 
 
 class SharedPrefixWorkspace:
@@ -476,9 +498,10 @@ class SharedPrefixWorkspace:
         self._buffer = torch.empty(0, dtype=torch.float32, device=device)
 
     def parts(self, rows: int, dim: int, prefix_splits: int, splits: int) -> tuple:
-        """Addresses of prefix_out, prefix_lse, part_out, part_lse for `rows` (row, head)s."""
+        """Addresses of prefix_out, prefix_lse, part_out, part_lse for `rows` (row, head)s,
+        and of the work counters."""
         sizes = [-(-n // 4) * 4 for n in (rows * prefix_splits * dim, rows * prefix_splits,
-                                          rows * splits * dim, rows * splits)]
+                                          rows * splits * dim, rows * splits, rows // 1024 + 1)]
         if self._buffer.numel() < sum(sizes):
             self._buffer = torch.empty(sum(sizes), dtype=torch.float32, device=self.device)
         at = self._buffer.data_ptr()
@@ -496,15 +519,15 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
                             workspace: SharedPrefixWorkspace | None = None,
                             out: torch.Tensor | None = None,
                             lse_out: torch.Tensor | None = None,
-                            seq_order: torch.Tensor | None = None,
+                            pages_per_split: int | None = None,
                             sms: int | None = None) -> torch.Tensor:
     """paged_decode_attention where groups of sequences share the pages of a prefix: these
     are read once for a group (tensor cores, up to 128 (sequence, head) rows together).
 
     max_suffix_pages / total_suffix_pages (host-known): the most pages any sequence has
     past its shared ones, and their sum over the batch (whole sequences where there is no
-    group); when omitted the block-table width bounds them. seq_order as in
-    paged_decode_attention. lse_out [B * Hq] fp32. bf16 pools only.
+    group); when omitted the block-table width bounds them. lse_out [B * Hq] fp32. bf16
+    pools only. Calls that share a workspace must not overlap on the GPU.
     """
     if kv_pool.dtype != torch.bfloat16:
         raise TypeError("shared_prefix_attention takes bf16 pools")
@@ -524,9 +547,9 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
         return paged_decode_attention(q, kv_pool, block_table, ctx_len, scale,
                                       max_pages_in_batch=max_suffix_pages,
                                       total_pages=total_suffix_pages, out=out, lse_out=lse_out,
-                                      seq_order=seq_order, sms=sms)
-    pps, nsplit = decode_plan(B, hq, hkv, max_suffix_pages or max_pages, None,
-                              total_suffix_pages, sms or sm_count(q.device))
+                                      sms=sms)
+    pps, nsplit = tail_split_plan(B, hq, hkv, max_suffix_pages or max_pages, pages_per_split,
+                                  total_suffix_pages, sms or sm_count(q.device))
     if out is None:
         out = torch.empty((B, hq, dim), dtype=torch.bfloat16, device=q.device)
     else:
@@ -537,18 +560,14 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
         require_cuda("lse_out", lse_out, torch.float32, 1, align=4)
         if lse_out.shape[0] != B * hq:
             raise ValueError("shared_prefix_attention: lse_out must be [B * Hq]")
-    if seq_order is not None:
-        require_cuda("seq_order", seq_order, torch.int32, 1, align=4)
-        if seq_order.shape[0] != B:
-            raise ValueError("shared_prefix_attention: seq_order needs one entry per sequence")
     if workspace is None:
         workspace = SharedPrefixWorkspace(q.device)
-    pre_out, pre_lse, part_out, part_lse = workspace.parts(B * hq, dim, groups.num_splits, nsplit)
+    pre_out, pre_lse, part_out, part_lse, counters = workspace.parts(B * hq, dim, groups.num_splits, nsplit)
     _capi.call("sc_shared_prefix_attention", ptr(q), ptr(kv_pool), num_pages, ptr(block_table),
-               ptr(ctx_len), ptr(seq_order), ptr(groups.first_page), ptr(groups.tiles),
+               ptr(ctx_len), ptr(groups.first_page), ptr(groups.tiles),
                ptr(groups.members), groups.ntiles, B, hq, hkv, dim, page, max_pages,
                groups.pages_per_split, groups.num_splits, pps, nsplit, float(scale), pre_out,
-               pre_lse, part_out, part_lse, ptr(out), ptr(lse_out), stream_of(q))
+               pre_lse, part_out, part_lse, counters, ptr(out), ptr(lse_out), stream_of(q))
     _count(3 if B else 0)
     return out
 
