@@ -556,7 +556,7 @@ int sc_shared_prefix_attention(const sc_bf16* q, const sc_bf16* kv_pool, int64_t
  *               -inf, the entries of lowest index follow with -inf
  * workspace     sc_beam_select_workspace bytes, 256-byte aligned
  * Supported: beams <= 64, n <= 64, beams * vocab < 2^31, groups * beams <= 65535. */
-size_t sc_beam_select_workspace(int groups, int beams, int vocab, int logits_fp32);
+size_t sc_beam_select_workspace(int groups, int beams, int vocab, int n, int logits_fp32);
 int sc_beam_select(const void* logits, int logits_fp32, int64_t row_stride, const float* scores,
                    const uint8_t* finished, int pad_token, float* out_scores, int32_t* parents,
                    int32_t* tokens, void* workspace, size_t workspace_bytes, int groups,
@@ -569,12 +569,12 @@ int sc_beam_select(const void* logits, int logits_fp32, int64_t row_stride, cons
  * slots[g][k]; child j continues beam parents[g][j]. The first child of a beam keeps
  * its row; each later child takes, in ascending order, the row of a beam without
  * children, and the parent's row is copied there in every layer of every pool.
- * slots, parents, new_slots [groups, beams] int32 (slots distinct); copies: scratch of
- * 2 + 2 * groups * beams int32, 8-byte aligned. A parent outside [0, beams) or a slot
- * outside [0, rows) is flagged (DEV_BAD_INDEX), and nothing is copied for it. beams <= 64. */
+ * slots, parents, new_slots [groups, beams] int32 (slots distinct; new_slots apart from
+ * the other two). A parent outside [0, beams) or a slot outside [0, rows) is flagged
+ * (DEV_BAD_INDEX), and nothing is copied for it. beams <= 64. */
 int sc_reorder_rows(void* const* pools, const int64_t* row_bytes, const int* layers, int npools,
                     int rows, const int32_t* slots, const int32_t* parents, int32_t* new_slots,
-                    int32_t* copies, int groups, int beams, void* stream);
+                    int groups, int beams, void* stream);
 
 #ifdef __cplusplus
 }

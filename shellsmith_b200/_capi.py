@@ -67,10 +67,10 @@ SIGNATURES = {
                          _I, _I, _I, _I, _I, _I64, _P],
     "sc_shared_prefix_attention": [_P, _P, _I64, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
                                    _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P, _P, _P, _P],
-    "sc_beam_select_workspace": [_I, _I, _I, _I],
+    "sc_beam_select_workspace": [_I, _I, _I, _I, _I],
     "sc_beam_select": [_P, _I, _I64, _P, _P, _I, _P, _P, _P, _P, ctypes.c_size_t, _I, _I, _I, _I,
                        _P],
-    "sc_reorder_rows": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _I, _I, _P],
+    "sc_reorder_rows": [_P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _P],
 }
 
 
@@ -115,6 +115,20 @@ def last_error() -> str:
     buf = ctypes.create_string_buffer(512)
     lib().sc_last_error(buf, len(buf))
     return buf.value.decode(errors="replace")
+
+
+def bind(name: str):
+    """A caller of one entry point, for wrappers whose own cost counts: looks the function
+    up once and raises as call() does."""
+    fn = None
+
+    def run(*args):
+        nonlocal fn
+        if fn is None:
+            fn = getattr(lib(), name)
+        if fn(*args):
+            raise ShellcacheError(name, lib().sc_last_error(None, 0), last_error())
+    return run
 
 
 def call(name: str, *args) -> None:

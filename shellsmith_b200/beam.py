@@ -14,6 +14,7 @@ page tables (engine.HybridCacheEngine.reorder).
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -23,6 +24,15 @@ from ._torch import ptr, require_cuda, stream_of
 
 MAX_BEAMS = 64   # beams of one group
 MAX_SELECT = 64  # continuations asked for at once
+
+_select = _capi.bind("sc_beam_select")
+_reorder = _capi.bind("sc_reorder_rows")
+_Pointers, _Sizes, _Layers = ctypes.c_void_p * 4, ctypes.c_int64 * 4, ctypes.c_int * 4
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(groups: int, beams: int, vocab: int, n: int, fp32: int) -> int:
+    return _capi.lib().sc_beam_select_workspace(groups, beams, vocab, n, fp32)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, *,
@@ -59,16 +69,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, *,
     if beams < 1 or vocab < 1:
         raise ValueError("beam_select: at least one beam and one token")
     fp32 = int(logits.dtype == torch.float32)
-    need = _capi.lib().sc_beam_select_workspace(groups, beams, vocab, fp32)
-    device = logits.device
-    work = torch.empty(need, dtype=torch.uint8, device=device)
-    best = torch.empty((groups, n), dtype=torch.float32, device=device)
-    where = torch.empty((2, groups, n), dtype=torch.int32, device=device)
-    parents, tokens = where[0], where[1]
+    need = _workspace(groups, beams, vocab, n, fp32)
+    work = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    best = scores.new_empty((groups, n))
+    parents, tokens = torch.empty((2, groups, n), dtype=torch.int32, device=logits.device).unbind(0)
     stride = logits.stride(1) if beams > 1 else (logits.stride(0) if groups > 1 else vocab)
-    _capi.call("sc_beam_select", ptr(logits), fp32, max(stride, vocab), ptr(scores), ptr(finished),
-               int(pad_token), ptr(best), ptr(parents), ptr(tokens), ptr(work), need, groups, beams,
-               vocab, int(n), stream_of(logits))
+    _select(logits.data_ptr(), fp32, max(stride, vocab), scores.data_ptr(), ptr(finished),
+            pad_token, best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), work.data_ptr(), need,
+            groups, beams, vocab, n, stream_of(logits))
     return best, parents, tokens
 
 
@@ -83,29 +91,27 @@ def reorder_rows(pools, slots: torch.Tensor, parents: torch.Tensor) -> torch.Ten
     """
     require_cuda("slots", slots, torch.int32, 2, align=4)
     require_cuda("parents", parents, torch.int32, 2, align=4)
-    if slots.shape != parents.shape:
+    groups, beams = shape = slots.shape
+    if parents.shape != shape:
         raise ValueError("reorder_rows: slots and parents must have the same shape")
-    groups, beams = slots.shape
-    pools = list(pools)
-    if len(pools) > 4:
-        raise ValueError(f"reorder_rows: at most 4 pools, got {len(pools)}")
-    rows = None
+    count = len(pools)
+    if count > 4:
+        raise ValueError(f"reorder_rows: at most 4 pools, got {count}")
+    rows, bases, sizes, layers = None, _Pointers(), _Sizes(), _Layers()
     for i, pool in enumerate(pools):
         if not isinstance(pool, torch.Tensor) or not pool.is_cuda or pool.dim() < 2:
             raise ValueError(f"reorder_rows: pool {i} must be a CUDA tensor [layers, rows, ...]")
         if not pool.is_contiguous():
             raise ValueError(f"reorder_rows: pool {i} must be contiguous")
-        if rows not in (None, pool.shape[1]):
+        size = pool.shape
+        if rows is not None and rows != size[1]:
             raise ValueError("reorder_rows: every pool must have the same rows")
-        rows = pool.shape[1]
-    count = len(pools)
-    bases = (ctypes.c_void_p * 4)(*(p.data_ptr() for p in pools))
-    sizes = (ctypes.c_int64 * 4)(*(p.stride(1) * p.element_size() for p in pools))
-    layers = (ctypes.c_int * 4)(*(p.shape[0] for p in pools))
+        rows = size[1]
+        bases[i], layers[i] = pool.data_ptr(), size[0]
+        sizes[i] = pool.stride(1) * pool.element_size()
     out = torch.empty_like(slots)
-    work = torch.empty(2 + 2 * slots.numel(), dtype=torch.int32, device=slots.device)
-    _capi.call("sc_reorder_rows", bases, sizes, layers, count, rows or 1, ptr(slots), ptr(parents),
-               ptr(out), ptr(work), groups, max(beams, 1), stream_of(slots))
+    _reorder(bases, sizes, layers, count, rows or 1, slots.data_ptr(), parents.data_ptr(),
+             out.data_ptr(), groups, beams or 1, stream_of(slots))
     return out
 
 

@@ -9,21 +9,31 @@
 // ascending), an order without ties. A NaN score counts as -inf. A finished beam
 // offers one candidate, (pad token, score_k).
 //
-// B200 mapping: HBM-bound, the logits are read once. scan_kernel: a CTA holds a chunk
-// of one row in registers, makes the chunk's (max, sum) and keeps every logit at or
-// above a threshold that at least n + 1 of the chunk reach: the (n + 1)-th largest of
-// its 256 threads' maxima (n + 1 distinct logits reach it; found by bisection over
-// the order-preserving integer keys, one block count per bit). Within a row the score
-// is monotone in the logit, so no other logit can be among the n best, save by the
-// rounding of scores below. merge_kernel, one CTA per group: the rows' statistics,
-// the scores of all kept logits, a threshold over them in the same way, and the rank
-// of each survivor by counting.
+// B200 mapping: HBM-bound, the logits are read once. scan_kernel: a CTA streams a segment
+// of one row, each warp every eighth block of 4 x 16 bytes a lane, the next block's loads
+// in flight while one is summed. Every lane keeps its own running maximum and sum. Beside
+// them the CTA keeps a list of granules (16 bytes of logits), to which its warps add
+// without waiting for one another: those whose maximum is not below a bound that n + 1
+// logits have reached, so that most granules cost their maximum and one comparison. A
+// warp starts with the (n + 1)-th largest of its first block's 128 maxima; whenever the
+// list has grown, the warp that notices takes the (n + 1)-th largest maximum of its newest
+// entries as the next bound. Both bisect over order-preserving integer keys by ballots. At
+// the segment's end the listed granules' logits are cut to the n + 1 largest. Within a row
+// the score is monotone in the logit, so no other logit can be among the n best, save by
+// the rounding of scores below. merge_kernel, one CTA per group: the rows' statistics, the
+// scores of all segments' candidates, a threshold over them in the same way, and the rank
+// of each survivor.
+//
+// Equal logits: of the granules whose maximum equals a warp's first bound its first block
+// keeps the n + 1 of lowest index and later blocks, whose indices are higher, none, so a
+// row masked with one value costs nothing. A list that overflows all the same (long runs
+// of one large value) is made anew, block by block in index order (ordered_list).
 //
 // Scores of different logits can round to the same fp32 number (a large |score_k|),
-// and then the lower index wins even against a larger logit. A chunk's dropped logits
-// are all below its threshold t; if the next value below t still scores as much as
-// the n-th best, merge_kernel rescans the group's logits for scores equal to it, in
-// index order, until it has enough.
+// and then the lower index wins even against a larger logit. A segment's dropped logits
+// are at most its last kept one t, and one equal to t has a higher index; if the next
+// value below t still scores as much as the n-th best, merge_kernel rescans the group's
+// logits for scores equal to it, in index order, until it has enough.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -32,11 +42,17 @@ namespace sc {
 namespace {
 
 constexpr int kScanThreads = 256;
-constexpr int kMergeThreads = 512;
+constexpr int kMergeThreads = 256;
 constexpr int kMaxSelect = 64;       // n
-constexpr int kSegment = 160;        // kept logits of one chunk (>= kMaxSelect + 1)
-constexpr int kScanList = 4096 + 80; // a chunk's survivors before they are cut to kSegment
-constexpr int kMergeList = 2048;
+constexpr int kScanWarps = kScanThreads / 32;
+constexpr int kVecs = 4;             // 16-byte loads of a lane per block
+constexpr int kScanList = kMaxSelect + 1 + kScanThreads * 8 + 63;  // n + 1 and a load a lane
+constexpr int kSegWaves = 4;         // segments per SM, all resident
+constexpr int kGranules = 512;       // listed granules
+constexpr int kNewest = 128;         // list entries that make a bound
+constexpr int kRankList = 256;       // lists up to here are ranked in one go
+constexpr int kMergeCache = 4096;    // candidates whose keys merge_kernel keeps
+constexpr int kMergeList = 1024;
 constexpr int kMaxBeams = 64;
 
 // Order-preserving unsigned keys of finite values and +inf; 0 for -inf and NaN.
@@ -61,6 +77,11 @@ template <>
 struct Logits<uint16_t> {  // bf16
   static constexpr int kPerVec = 8;
   static constexpr int kBits = 16;  // significant high bits of a key
+  __device__ static float largest(const uint4& u) {  // NaN only where all are
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
   __device__ static float value(uint16_t x) { return bf16_to_f(x); }
   __device__ static float get(const uint4& u, int e) {
     const uint32_t w = e < 2 ? u.x : e < 4 ? u.y : e < 6 ? u.z : u.w;
@@ -82,6 +103,9 @@ template <>
 struct Logits<float> {
   static constexpr int kPerVec = 4;
   static constexpr int kBits = 32;
+  __device__ static float largest(const uint4& u) {
+    return fmaxf(fmaxf(get(u, 0), get(u, 1)), fmaxf(get(u, 2), get(u, 3)));
+  }
   __device__ static float value(float x) { return x; }
   __device__ static float get(const uint4& u, int e) {
     return __uint_as_float(e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w);
@@ -96,6 +120,26 @@ struct Logits<float> {
   __device__ static float below(float x) { return unkey(key(x) - 1u); }
 };
 
+// Two fp32 lanes in one register pair: one instruction for two sums or products.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // (max, sum of e^(x - max)) of two disjoint sets. A NaN sum stays NaN; a set whose
 // maximum is -inf is empty unless its sum is NaN.
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
@@ -106,17 +150,53 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   s = a + b;
 }
 
-// Largest key t (its low 32 - kBits bits zero) such that at least `want` threads hold
-// a key >= t; 0 when fewer than `want` hold any. Bits are set from the top.
+// Cuts the CTA's list (unsorted, `total` > `want` entries) to its `want` largest keys,
+// equal ones by the lower index, in place; returns the smallest key left. The key by
+// bisection; of a run of equal ones as many as fit stay, the lowest indices first.
 template <int kBits>
-__device__ __forceinline__ uint32_t nth_key(uint32_t key, int want) {
-  uint32_t t = 0;
+__device__ uint32_t cut_list(uint32_t* list_k, int* list_v, int total, int want, int* scratch) {
+  uint32_t cut = 0u;
 #pragma unroll 1
   for (int b = 31; b >= 32 - kBits; --b) {
-    const uint32_t next = t | (1u << b);
-    if (__syncthreads_count(key >= next) >= want) t = next;
+    const uint32_t next = cut | (1u << b);
+    int c = 0;
+    for (int i = threadIdx.x; i < total; i += kScanThreads) c += list_k[i] >= next;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = c;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < kScanThreads / 32; ++w) all += scratch[w];
+    if (all >= want) cut = next;
+    __syncthreads();
   }
-  return t;
+  constexpr int kMost = (kScanList + kScanThreads - 1) / kScanThreads;
+  uint32_t k[kMost];
+  int v[kMost];
+  uint32_t keep = 0u;
+#pragma unroll
+  for (int j = 0; j < kMost; ++j) {
+    const int i = threadIdx.x + j * kScanThreads;
+    k[j] = i < total ? list_k[i] : 0u;
+    v[j] = i < total ? list_v[i] : 0;
+    if (i >= total || k[j] < cut) continue;
+    int before = 0;
+    if (k[j] == cut)
+      for (int o = 0; o < total; ++o)
+        before += list_k[o] > cut || (list_k[o] == cut && list_v[o] < v[j]);
+    if (before < want) keep |= 1u << j;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) scratch[0] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kMost; ++j)
+    if (keep >> j & 1u) {
+      const int at = atomicAdd(&scratch[0], 1);
+      list_k[at] = k[j];
+      list_v[at] = v[j];
+    }
+  __syncthreads();
+  return cut;
 }
 
 struct SelectArgs {
@@ -124,14 +204,12 @@ struct SelectArgs {
   long long row_stride;          // elements between rows
   const float* scores;           // [G, K]
   const uint8_t* finished;       // [G, K] or NULL
-  float2* stats;                 // [rows][chunks] (max, sum)
-  int* counts;                   // [rows][chunks] kept
-  float* floors;                 // [rows][chunks] threshold where logits were dropped, else -inf
-  float* kept_x;                 // [rows][chunks][kSegment]
-  int32_t* kept_v;
+  float2* stats;                 // [rows][segs] (max, sum)
+  float* floors;                 // [rows][segs] last kept logit where some were dropped, else -inf
+  uint2* kept;                   // [rows][segs][n + 1] (logit bits, token), -inf: none
   float* out_scores;             // [G, n]
   int32_t *parents, *tokens;
-  int G, K, V, n, chunks, pad;
+  int G, K, V, n, segs, seg_blocks, pad;
 };
 
 // A row that offers no logit: finished, or its score is -inf or NaN.
@@ -139,190 +217,314 @@ __device__ __forceinline__ bool row_idle(const SelectArgs& a, int row) {
   return (a.finished != nullptr && a.finished[row]) || !(a.scores[row] > -CUDART_INF_F);
 }
 
-template <typename T, int kVecs>
-__global__ void __launch_bounds__(kScanThreads) scan_kernel(const SelectArgs a) {
+// One of the warp's keys that at least `want` of them reach: the want-th largest, but for
+// at most 1/1024 of their span (which a bound may be below). 0 if fewer keys than that are
+// not 0. A lane holds kPer of them.
+template <int kPer>
+__device__ __forceinline__ uint32_t warp_nth(const uint32_t* k, int want) {
+  constexpr unsigned kAll = 0xffffffffu;
+  uint32_t hi = 0u, lo = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    hi = max(hi, k[i]);
+    lo = k[i] != 0u ? min(lo, k[i]) : lo;
+  }
+  hi = __reduce_max_sync(kAll, hi);
+  lo = __reduce_min_sync(kAll, lo);
+  const auto reach = [&](uint32_t t) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) c += k[i] >= t;
+    return (int)__reduce_add_sync(kAll, (unsigned)c);
+  };
+  if (reach(1u) < want) return 0u;
+  if (reach(hi) >= want) return hi;
+  uint32_t step = hi - lo;  // at least want keys reach lo, fewer reach lo + step
+#pragma unroll 1
+  for (int i = 0; i < 10 && step > 1u; ++i) {
+    const uint32_t half = step >> 1;
+    if (reach(lo + half) >= want) {
+      lo += half;
+      step -= half;
+    } else {
+      step = half;
+    }
+  }
+  uint32_t t = 0xffffffffu;  // the smallest key that reaches it, an actual one
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) t = k[i] >= lo ? min(t, k[i]) : t;
+  return __reduce_min_sync(kAll, t);
+}
+
+// (m, s) of the warp's lanes joined: one maximum, one rescaling and one sum.
+__device__ __forceinline__ void warp_join(float& m, float& s) {
+  constexpr unsigned kAll = 0xffffffffu;
+  const uint32_t b = __float_as_uint(m);
+  const uint32_t top = __reduce_max_sync(kAll, (b & 0x80000000u) ? ~b : (b | 0x80000000u));
+  const float M = key_value(top);
+  // An empty lane (s = 0) stays 0; a lane at the maximum is not rescaled (inf - inf).
+  s = s == 0.f || m == M ? s : s * expf(m - M);
+  m = M;
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(kAll, s, off);
+}
+
+// The candidates of granules [g_begin, g_end) in index order, the CTA in step: a tile of a
+// granule a thread at a time, the list cut whenever a tile might not fit. Returns its
+// length (at least min(want, candidates); cut_list does the rest).
+template <typename T>
+__device__ __noinline__ int ordered_list(const T* base, int lead, int V, int g_begin, int g_end,
+                                         uint32_t* list_k, int* list_v, int want, int* scratch,
+                                         int* n_list) {
   using L = Logits<T>;
   constexpr int E = L::kPerVec;
+  if (threadIdx.x == 0) *n_list = 0;
+  __syncthreads();
+  uint32_t bound = 0u;
+  for (int g0 = g_begin; g0 < g_end; g0 += kScanThreads) {
+    const int v0 = (g0 + (int)threadIdx.x) * E - lead;
+    uint32_t k[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      k[e] = g0 + (int)threadIdx.x < g_end && v0 + e >= 0 && v0 + e < V ? L::key(L::value(base[v0 + e]))
+                                                                       : 0u;
+    if (*n_list > 2 * want) {  // uniform
+      const int total = *n_list;
+      bound = max(bound, cut_list<L::kBits>(list_k, list_v, total, want, scratch));
+      if (threadIdx.x == 0) *n_list = want;
+      __syncthreads();
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (k[e] > bound) {
+        const int at = atomicAdd(n_list, 1);
+        list_k[at] = k[e];
+        list_v[at] = v0 + e;
+      }
+    __syncthreads();
+  }
+  return *n_list;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const SelectArgs a) {
+  using L = Logits<T>;
+  constexpr int E = L::kPerVec;
+  constexpr float kLog2e = 1.4426950408889634f;
+  constexpr unsigned kAll = 0xffffffffu;
+  constexpr int kBlock = 32 * kVecs;  // granules of a warp's block
+  __shared__ uint4 gran[kGranules];          // listed granules, their first element's index
+  __shared__ int gran_v[kGranules];          // and the key of their maximum
+  __shared__ uint32_t gran_k[kGranules];
   __shared__ uint32_t list_k[kScanList];
   __shared__ int list_v[kScanList];
-  __shared__ int n_above, n_equal, n_out;
-  __shared__ float red_m[kScanThreads / 32], red_s[kScanThreads / 32];
-  __shared__ int scan_w[kScanThreads / 32];
+  __shared__ uint32_t shared_bound;          // n + 1 logits of the segment reach it
+  __shared__ int n_gran, n_list, refresh_at;
+  __shared__ float red_m[kScanWarps], red_s[kScanWarps];
+  __shared__ int scratch[kScanWarps];
   pdl_wait();
   pdl_trigger();
-  const int row = blockIdx.y, chunk = blockIdx.x;
-  const size_t seg = (size_t)row * a.chunks + chunk;
-  if (row_idle(a, row)) {  // uniform over the CTA
-    if (threadIdx.x == 0) {
-      a.counts[seg] = 0;
-      a.floors[seg] = -CUDART_INF_F;
-    }
-    return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = blockIdx.y, want = a.n + 1;
+  const size_t seg = (size_t)row * a.segs + blockIdx.x;
+  if (row_idle(a, row)) return;  // uniform over the CTA; merge_kernel skips the row too
+  for (int i = tid; i < kGranules; i += kScanThreads) gran_k[i] = 0u;  // 0: not written yet
+  if (tid == 0) {
+    shared_bound = 0u;
+    n_gran = n_list = 0;
+    refresh_at = 2 * want;
   }
-  if (threadIdx.x == 0) n_above = n_equal = n_out = 0;
+  __syncthreads();
   // Aligned 16-byte granules over the row; the first and the last may hold elements
   // outside it, which are read one by one.
   const T* base = reinterpret_cast<const T*>(a.logits) + (long long)row * a.row_stride;
   const int lead = (int)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
   const T* start = base - lead;  // granule g covers elements E g - lead .. of the row
-  const int g0 = chunk * kScanThreads * kVecs + threadIdx.x;
-  uint4 r[kVecs];
+  const int granules = (a.V + lead + E - 1) / E;
+  const int g_begin = (int)blockIdx.x * a.seg_blocks * kScanWarps * kBlock;
+  const int g_end = min(granules, g_begin + a.seg_blocks * kScanWarps * kBlock);
+  int g0 = g_begin + warp * kBlock + lane;
+  const auto load = [&](int g, uint4* r) {
+    if (g - lane + kBlock <= g_end && (g - lane) * E - lead >= 0 &&
+        (g - lane + kBlock) * E - lead <= a.V) {  // uniform: a whole block
 #pragma unroll
-  for (int j = 0; j < kVecs; ++j) {
-    const int v0 = (g0 + j * kScanThreads) * E - lead;
-    if (v0 >= 0 && v0 + E <= a.V) {
-      r[j] = __ldcs(reinterpret_cast<const uint4*>(start) + g0 + j * kScanThreads);
+      for (int j = 0; j < kVecs; ++j)
+        r[j] = __ldcs(reinterpret_cast<const uint4*>(start) + g + 32 * j);
     } else {
-      r[j] = L::fill();
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (v0 + e >= 0 && v0 + e < a.V) L::put(r[j], e, base[v0 + e]);
+      for (int j = 0; j < kVecs; ++j) {
+        const int gj = g + 32 * j, v0 = gj * E - lead;
+        r[j] = L::fill();
+        if (gj < g_end)
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (v0 + e >= 0 && v0 + e < a.V) L::put(r[j], e, base[v0 + e]);
+      }
     }
-  }
-  float m = -CUDART_INF_F, s = 0.f;
-#pragma unroll
-  for (int j = 0; j < kVecs; ++j)
-#pragma unroll
-    for (int e = 0; e < E; ++e) m = fmaxf(m, L::get(r[j], e));
-  // x - m is taken before the change of base: the largest terms then carry no error of
-  // the product with log2 e. Where every x is -inf (or NaN) the sum tells them apart.
-  const float ref = m == -CUDART_INF_F ? 0.f : m;
-#pragma unroll
-  for (int j = 0; j < kVecs; ++j)
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += ex2((L::get(r[j], e) - ref) * 1.4426950408889634f);
-
-  const uint32_t mine = L::key(m);
-  const uint32_t t = nth_key<L::kBits>(mine, a.n + 1);
-  // Logits above t: at most n threads hold any, so they fit the list.
-  const auto push = [&](int at, uint32_t k, int j, int e) {
-    list_k[at] = k;
-    list_v[at] = (g0 + j * kScanThreads) * E - lead + e;
   };
-  int eq = 0;
-  if (mine >= t && mine != 0u) {
+  // This lane's maximum and the sum of e^(x - m). x - m comes before the change of base: a
+  // product with log2 e would add its rounding to the largest terms (and overflow at the
+  // type's ends).
+  float m = -CUDART_INF_F, s = 0.f;
+  float own = -CUDART_INF_F;  // this warp's first bound: later granules count above it
+  bool first = true;
+  constexpr int kRound = kScanWarps * kBlock;
+  uint4 r[kVecs], next[kVecs];
+  load(g0, r);
+#pragma unroll 1
+  for (; g0 - lane < g_end; g0 += kRound) {
+    load(g0 + kRound, next);
+    float top[kVecs];
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) top[j] = L::largest(r[j]);
+    float all = top[0];
+#pragma unroll
+    for (int j = 1; j < kVecs; ++j) all = fmaxf(all, top[j]);
+    if (all > m) {
+      s *= m == -CUDART_INF_F ? 1.f : ex2((m - all) * kLog2e);  // a NaN sum stays
+      m = all;
+    }
+    const float shift = m == -CUDART_INF_F ? 0.f : -m;
+    uint64_t sums[2] = {pair(s, 0.f), pair(0.f, 0.f)};
 #pragma unroll
     for (int j = 0; j < kVecs; ++j)
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const uint32_t k = L::key(L::get(r[j], e));
-        if (k > t) push(atomicAdd(&n_above, 1), k, j, e);
-        eq += k == t && t != 0u;
+      for (int e = 0; e < E; e += 2) {
+        float y0, y1;
+        unpair(mul2(add2(pair(L::get(r[j], e), L::get(r[j], e + 1)), pair(shift, shift)),
+                    pair(kLog2e, kLog2e)),
+               y0, y1);
+        sums[e / 2 % 2] = add2(sums[e / 2 % 2], pair(ex2(y0), ex2(y1)));
       }
-    if (eq) atomicAdd(&n_equal, eq);
-  }
-  float wm = m, ws = s;
+    float s0, s1;
+    unpair(add2(sums[0], sums[1]), s0, s1);
+    s = s0 + s1;
+    unsigned hot = 0u;  // granules of this lane that go on the list
+    if (!first) {
+      const uint32_t least_k = *reinterpret_cast<volatile uint32_t*>(&shared_bound);
+      const float least = least_k == 0u ? -CUDART_INF_F : L::unkey(least_k);
+      if (__any_sync(kAll, all > own && all >= least)) {
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, wm, off);
-    const float s2 = __shfl_xor_sync(0xffffffffu, ws, off);
-    join(wm, ws, m2, s2);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    red_m[threadIdx.x >> 5] = wm;
-    red_s[threadIdx.x >> 5] = ws;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kScanThreads / 32; ++w) join(wm, ws, red_m[w], red_s[w]);
-    a.stats[seg] = make_float2(wm, ws);
-  }
-  const int above = n_above, equal = n_equal;
-  int total = above + equal;
-  if (total <= kSegment) {
-    if (eq) {
+        for (int j = 0; j < kVecs; ++j) hot |= (top[j] > own && top[j] >= least) ? 1u << j : 0u;
+      }
+    } else {
+      first = false;
+      uint32_t k[kVecs];
 #pragma unroll
-      for (int j = 0; j < kVecs; ++j)
+      for (int j = 0; j < kVecs; ++j) k[j] = L::key(top[j]);
+      const uint32_t t = warp_nth<kVecs>(k, want);
+      if (t != 0u) own = L::unkey(t);
+      if (lane == 0) atomicMax(&shared_bound, t);
+      int equals = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (L::key(L::get(r[j], e)) == t) push(above + atomicAdd(&n_out, 1), t, j, e);
+      for (int j = 0; j < kVecs; ++j) {
+        const unsigned eq = __ballot_sync(kAll, k[j] == t && t != 0u);
+        const int rank = equals + __popc(eq & ((1u << lane) - 1u));
+        hot |= (k[j] > t || ((eq >> lane & 1u) && rank < want)) ? 1u << j : 0u;
+        equals += __popc(eq);
+      }
     }
-  } else {
-    // Of the equal ones the n + 1 of lowest index are enough: any other has as much as
-    // these and comes after them. Granule j of the threads in order is index order.
-    int have = 0;
+    if (__any_sync(kAll, hot != 0u)) {
+      if (hot != 0u) {
+        int at = atomicAdd(&n_gran, __popc(hot));
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) {
-      if (have > a.n) break;  // uniform
-      int c = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) c += t != 0u && L::key(L::get(r[j], e)) == t;
-      int incl = c;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, off);
-        if ((threadIdx.x & 31) >= off) incl += y;
+        for (int j = 0; j < kVecs; ++j)
+          if (hot >> j & 1u) {
+            if (at < kGranules) {  // an overflow is seen at the end
+              gran[at] = r[j];
+              gran_v[at] = (g0 + 32 * j) * E - lead;
+              gran_k[at] = L::key(top[j]);
+            }
+            ++at;
+          }
       }
-      if ((threadIdx.x & 31) == 31) scan_w[threadIdx.x >> 5] = incl;
-      __syncthreads();
-      int at = have + incl - c, sum = 0;
-      for (int w = 0; w < kScanThreads / 32; ++w) {
-        if (w < (int)(threadIdx.x >> 5)) at += scan_w[w];
-        sum += scan_w[w];
+      // Has the list grown enough for a better bound, and is it this warp that makes it?
+      int now = 0;
+      if (lane == 0) {
+        now = *reinterpret_cast<volatile int*>(&n_gran);
+        const int due = *reinterpret_cast<volatile int*>(&refresh_at);
+        if (now < due || atomicCAS(&refresh_at, due, now + want) != due) now = 0;
       }
+      now = min(__shfl_sync(kAll, now, 0), kGranules);
+      if (now != 0) {
+        uint32_t k[kNewest / 32];
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (t != 0u && L::key(L::get(r[j], e)) == t) {
-          if (at <= a.n) push(above + at, t, j, e);
-          ++at;
+        for (int i = 0; i < kNewest / 32; ++i) {
+          const int at = now - 1 - lane - 32 * i;
+          k[i] = at >= 0 ? *reinterpret_cast<volatile uint32_t*>(&gran_k[at]) : 0u;
         }
-      have += sum;
-      __syncthreads();
-    }
-    total = above + min(have, a.n + 1);
-  }
-  __syncthreads();
-  // Cut to the segment: the n + 1 largest (equal ones: lowest index) of the list.
-  uint32_t cut = t;
-  if (total > kSegment) {
-    cut = 0;
-#pragma unroll 1
-    for (int b = 31; b >= 32 - L::kBits; --b) {
-      const uint32_t next = cut | (1u << b);
-      int c = 0;
-      for (int i = threadIdx.x; i < total; i += kScanThreads) c += list_k[i] >= next;
-      c = __reduce_add_sync(0xffffffffu, c);
-      if ((threadIdx.x & 31) == 0) scan_w[threadIdx.x >> 5] = c;
-      __syncthreads();
-      int all = 0;
-      for (int w = 0; w < kScanThreads / 32; ++w) all += scan_w[w];
-      if (all > a.n) cut = next;
-      __syncthreads();
-    }
-    if (threadIdx.x == 0) n_out = 0;
-    __syncthreads();
-  }
-  float* kx = a.kept_x + seg * kSegment;
-  int32_t* kv = a.kept_v + seg * kSegment;
-  if (total <= kSegment) {
-    for (int i = threadIdx.x; i < total; i += kScanThreads) {
-      kx[i] = L::unkey(list_k[i]);
-      kv[i] = list_v[i];
-    }
-  } else {
-    for (int i = threadIdx.x; i < total; i += kScanThreads) {
-      const uint32_t k = list_k[i];
-      bool keep = k > cut;
-      if (k == cut) {  // rank among the equal ones and those above
-        int rank = 0;
-        for (int o = 0; o < total; ++o) rank += list_k[o] > cut || (list_k[o] == cut && list_v[o] < list_v[i]);
-        keep = rank <= a.n;
-      }
-      if (keep) {
-        const int at = atomicAdd(&n_out, 1);
-        kx[at] = L::unkey(k);
-        kv[at] = list_v[i];
+        const uint32_t t = warp_nth<kNewest / 32>(k, want);
+        if (lane == 0) atomicMax(&shared_bound, t);
       }
     }
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) r[j] = next[j];
+  }
+  warp_join(m, s);
+  if (lane == 0) {
+    red_m[warp] = m;
+    red_s[warp] = s;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    a.counts[seg] = total <= kSegment ? total : n_out;
-    a.floors[seg] = cut == 0u ? -CUDART_INF_F : L::unkey(cut);  // 0: every candidate is kept
+  // The listed granules' logits that are not below the last bound.
+  const int grans = n_gran;
+  const uint32_t least = max(shared_bound, 1u);
+  for (int i = tid; i < min(grans, kGranules); i += kScanThreads) {
+    if (gran_k[i] < least) continue;
+    const uint4 g = gran[i];
+    uint32_t key[E];
+    unsigned hits = 0u;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      key[e] = L::key(L::get(g, e));
+      hits |= key[e] >= least ? 1u << e : 0u;
+    }
+    int at = atomicAdd(&n_list, __popc(hits));
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (hits >> e & 1u) {
+        if (at < kScanList) {
+          list_k[at] = key[e];
+          list_v[at] = gran_v[i] + e;
+        }
+        ++at;
+      }
+  }
+  __syncthreads();
+  int total = n_list;
+  __syncthreads();
+  if (grans > kGranules || total > kScanList)
+    total = ordered_list(base, lead, a.V, g_begin, g_end, list_k, list_v, want, scratch, &n_list);
+  if (total > kRankList) {
+    cut_list<L::kBits>(list_k, list_v, total, want, scratch);
+    total = want;
+  }
+  // One entry a thread, ranked by counting the better ones; the n + 1 best go out in order.
+  uint2* kept = a.kept + seg * want;
+  const uint32_t key = tid < total ? list_k[tid] : 0u;
+  const int v = tid < total ? list_v[tid] : 0;
+  if (tid < total) {
+    int rank = 0;
+#pragma unroll 4
+    for (int o = 0; o < total; ++o) {
+      const uint32_t ko = list_k[o];
+      rank += ko > key || (ko == key && list_v[o] < v);
+    }
+    if (rank < want) kept[rank] = make_uint2(__float_as_uint(L::unkey(key)), (uint32_t)v);
+    // Where logits were dropped at all, n + 1 are left, and none dropped is above the last.
+    if (rank == a.n) a.floors[seg] = L::unkey(key);
+  }
+  for (int i = total + tid; i < want; i += kScanThreads) kept[i] = make_uint2(0xff800000u, 0u);
+  if (total < want && tid == 0) a.floors[seg] = -CUDART_INF_F;
+  if (warp == kScanWarps - 1) {
+    m = lane < kScanWarps ? red_m[lane] : -CUDART_INF_F;
+    s = lane < kScanWarps ? red_s[lane] : 0.f;
+    warp_join(m, s);
+    if (lane == 0) a.stats[seg] = make_float2(m, s);
   }
 }
 
-// The number of keys >= bound over the CTA's threads' items, for the bisections below.
+// Sum of c over the CTA.
 __device__ __forceinline__ int block_total(int c, int* scratch) {
   c = __reduce_add_sync(0xffffffffu, c);
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = c;
@@ -336,77 +538,101 @@ __device__ __forceinline__ int block_total(int c, int* scratch) {
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const SelectArgs a) {
   using L = Logits<T>;
-  __shared__ float row_m[kMaxBeams], row_l[kMaxBeams];
-  __shared__ unsigned long long list[kMergeList];
+  __shared__ float row_m[kMaxBeams], row_l[kMaxBeams], row_s[kMaxBeams];
+  __shared__ bool row_on[kMaxBeams];
+  __shared__ unsigned long long cache[kMergeCache], list[kMergeList];
   __shared__ int scratch[kMergeThreads / 32];
-  __shared__ int n_list, ambiguous;
+  __shared__ int n_list, ambiguous, strictly;
+  __shared__ uint32_t last_score, threshold, best_k[kMergeThreads];
   pdl_wait();
   pdl_trigger();
   const int g = blockIdx.x, K = a.K, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) n_list = ambiguous = 0;
+  if (threadIdx.x == 0) n_list = ambiguous = strictly = 0, last_score = 0u;
   for (int k = warp; k < K; k += kMergeThreads / 32) {
     const int row = g * K + k;
     float m = -CUDART_INF_F, s = 0.f;
-    if (!row_idle(a, row))
-      for (int c = lane; c < a.chunks; c += 32) {
-        const float2 st = a.stats[(size_t)row * a.chunks + c];
+    const bool on = !row_idle(a, row);
+    if (on)
+      for (int c = lane; c < a.segs; c += 32) {
+        const float2 st = a.stats[(size_t)row * a.segs + c];
         join(m, s, st.x, st.y);
       }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, off);
-      const float s2 = __shfl_xor_sync(0xffffffffu, s, off);
-      join(m, s, m2, s2);
-    }
+    warp_join(m, s);
     if (lane == 0) {
       row_m[k] = m;
       row_l[k] = logf(s);
+      row_s[k] = a.scores[row];
+      row_on[k] = on;
     }
   }
   __syncthreads();
-  const auto score = [&](int k, float x) {
-    return a.scores[g * K + k] + ((x - row_m[k]) - row_l[k]);
-  };
+  const auto score = [&](int k, float x) { return row_s[k] + ((x - row_m[k]) - row_l[k]); };
   // (score, lower index first) as one key; 0 for -inf and NaN.
   const auto full_key = [&](int k, float sc, int v) -> unsigned long long {
     const uint32_t key = score_key(sc);
     return key == 0u ? 0ull
                      : ((unsigned long long)key << 32) | (0xffffffffu - ((uint32_t)k * a.V + v));
   };
-  const int segs = K * a.chunks;
-  // Items: the kept logits of segment i / kSegment, then one per finished beam.
-  const auto each = [&](auto&& f) {
-    for (int sgm = warp; sgm < segs; sgm += kMergeThreads / 32) {
-      const int k = sgm / a.chunks;
-      const size_t seg = (size_t)g * segs + sgm;
-      const int cnt = a.counts[seg];
-      for (int i = lane; i < cnt; i += 32)
-        f(full_key(k, score(k, a.kept_x[seg * kSegment + i]), a.kept_v[seg * kSegment + i]));
+  // Items: the segments' candidates, then one per beam for the finished ones.
+  const int per = a.n + 1, segs = K * a.segs, cands = segs * per, items = cands + K;
+  const auto make = [&](int i) -> unsigned long long {
+    if (i >= cands) {
+      const int k = i - cands;
+      const bool fin = a.finished != nullptr && a.finished[g * K + k];
+      return fin ? full_key(k, row_s[k], a.pad) : 0ull;
     }
-    if (a.finished != nullptr)
-      for (int k = threadIdx.x; k < K; k += kMergeThreads)
-        if (a.finished[g * K + k]) f(full_key(k, a.scores[g * K + k], a.pad));
+    const int k = i / (a.segs * per);
+    if (!row_on[k]) return 0ull;
+    const uint2 c = a.kept[(size_t)g * cands + i];
+    return full_key(k, score(k, __uint_as_float(c.x)), (int)c.y);
   };
+  const bool cached = items <= kMergeCache;
   unsigned long long best = 0ull;
-  each([&](unsigned long long key) { best = key > best ? key : best; });
-  // At least n items reach the n-th largest of the threads' best scores.
-  uint32_t t = nth_key<32>((uint32_t)(best >> 32), a.n);
-  int c = 0;
-  each([&](unsigned long long key) { c += key != 0ull && (uint32_t)(key >> 32) >= t; });
+  for (int i = threadIdx.x; i < items; i += kMergeThreads) {
+    const unsigned long long key = make(i);
+    if (cached) cache[i] = key;
+    best = key > best ? key : best;
+  }
+  const auto item = [&](int i) { return cached ? cache[i] : make(i); };  // own items only
+  // At least n items reach about the n-th largest of the threads' best scores.
+  best_k[threadIdx.x] = (uint32_t)(best >> 32);
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t k[kMergeThreads / 32];
+#pragma unroll
+    for (int i = 0; i < kMergeThreads / 32; ++i) k[i] = best_k[lane + 32 * i];
+    const uint32_t bound = warp_nth<kMergeThreads / 32>(k, a.n);
+    if (lane == 0) threshold = bound;
+  }
+  __syncthreads();
+  const uint32_t t = threshold;
   unsigned long long floor_key = (unsigned long long)t << 32;
-  if (block_total(c, scratch) > kMergeList) {  // the n largest keys exactly
+  int c = 0;
+  if (best >= floor_key)
+    for (int i = threadIdx.x; i < items; i += kMergeThreads) {
+      const unsigned long long key = item(i);
+      if (key != 0ull && key >= floor_key) {
+        const int at = atomicAdd(&n_list, 1);
+        if (at < kMergeList) list[at] = key;
+      }
+    }
+  __syncthreads();
+  if (n_list > kMergeList) {  // the n largest keys exactly
     floor_key = 0ull;
     for (int b = 63; b >= 0; --b) {
       const unsigned long long next = floor_key | (1ull << b);
       c = 0;
-      each([&](unsigned long long key) { c += key >= next; });
+      for (int i = threadIdx.x; i < items; i += kMergeThreads) c += item(i) >= next;
       if (block_total(c, scratch) >= a.n) floor_key = next;
     }
+    if (threadIdx.x == 0) n_list = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < items; i += kMergeThreads) {
+      const unsigned long long key = item(i);
+      if (key != 0ull && key >= floor_key) list[atomicAdd(&n_list, 1)] = key;
+    }
+    __syncthreads();
   }
-  each([&](unsigned long long key) {
-    if (key != 0ull && key >= floor_key) list[atomicAdd(&n_list, 1)] = key;
-  });
-  __syncthreads();
   const int total = n_list;
   float* os = a.out_scores + (size_t)g * a.n;
   int32_t* op = a.parents + (size_t)g * a.n;
@@ -416,10 +642,6 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const SelectArgs a
     op[rank] = (int32_t)(flat / (uint32_t)a.V);
     ot[rank] = (int32_t)(flat % (uint32_t)a.V);
   };
-  __shared__ uint32_t last_score;
-  __shared__ int strictly;
-  if (threadIdx.x == 0) last_score = 0u, strictly = 0;
-  __syncthreads();
   for (int i = threadIdx.x; i < total; i += kMergeThreads) {
     const unsigned long long key = list[i];
     int rank = 0;
@@ -443,8 +665,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const SelectArgs a
   }
   // A dropped logit that rounds to the n-th best score may have a lower index.
   for (int sgm = threadIdx.x; sgm < segs; sgm += kMergeThreads) {
+    const int k = sgm / a.segs;
+    if (!row_on[k]) continue;
     const float fl = a.floors[(size_t)g * segs + sgm];
-    if (fl > -CUDART_INF_F && score_key(score(sgm / a.chunks, L::below(fl))) >= last) ambiguous = 1;
+    if (fl > -CUDART_INF_F && score_key(score(k, L::below(fl))) >= last) ambiguous = 1;
   }
   for (int i = threadIdx.x; i < total; i += kMergeThreads)
     if ((uint32_t)(list[i] >> 32) > last) atomicAdd(&strictly, 1);
@@ -454,9 +678,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const SelectArgs a
   int have = strictly;
   for (int k = 0; k < K && have < a.n; ++k) {
     const int row = g * K + k;
-    if (row_idle(a, row)) {
+    if (!row_on[k]) {
       const bool fin = a.finished != nullptr && a.finished[row];
-      if (fin && a.scores[row] == target) {
+      if (fin && row_s[k] == target) {
         if (threadIdx.x == 0) emit(have, target, (uint32_t)k * a.V + a.pad);
         ++have;
       }
@@ -481,16 +705,20 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const SelectArgs a
   }
 }
 
-// Chunks of 8 granules a thread amortise the bisection; small calls take 2, so that
-// their few rows spread over more SMs.
+// Segments of a row, in whole rounds of blocks (one a warp): as many as the GPU holds at
+// once, so that every segment is long and its first bound and its end pay.
+struct Segments {
+  int blocks, count;  // rounds of blocks per segment, segments per row
+};
 template <typename T>
-int select_vecs(long long rows, int V) {
-  return rows * V <= (long long)148 * kScanThreads * Logits<T>::kPerVec * 8 ? 2 : 8;
-}
-template <typename T>
-int chunk_count(int V, int vecs) {
-  const int per = kScanThreads * vecs * Logits<T>::kPerVec;
-  return (int)(((long long)V + Logits<T>::kPerVec - 1 + per - 1) / per);  // + the lead of an unaligned row
+Segments select_segments(long long rows, int V) {
+  const int per = kScanThreads * kVecs * Logits<T>::kPerVec;
+  const int rounds = (int)(((long long)V + Logits<T>::kPerVec - 1 + per - 1) / per);  // + the lead
+  const long long most = 148ll * kSegWaves / rows;
+  Segments s;
+  s.blocks = most >= rounds ? 1 : (int)((rounds + (most < 1 ? 1 : most) - 1) / (most < 1 ? 1 : most));
+  s.count = (rounds + s.blocks - 1) / s.blocks;
+  return s;
 }
 
 // ---------------------------------------------------------------- reordering of rows
@@ -498,123 +726,166 @@ int chunk_count(int V, int vecs) {
 // beam's slot; each later child takes the slot of a beam without children, in ascending
 // order of both. A slot that is read is never written, so the copies run in place and
 // in any order.
-constexpr int kPlanThreads = 256;
+//
+// One launch: every CTA makes the whole plan for itself (a warp a group, beams as 64-bit
+// masks; a few hundred cycles) and then takes its share of the places to copy, a place
+// being one source's 16 KB piece of a layer, read once and written to each of its
+// destinations. Larger batches make the plan in slices that fit shared memory.
 constexpr int kCopyThreads = 256;
-constexpr int kCopyVecs = 4;  // 16-byte loads in flight per thread
+constexpr int kCopyVecs = 4;       // 16-byte loads in flight per thread
+constexpr int kPlanBeams = 1024;   // beams planned at once
 
 struct ReorderPools {
   uint8_t* base[4];
   long long chunks[4];  // 16-byte chunks per row
-  int layers[4];
-  long long first[5];   // work units before pool p, per copied row
+  long long first[5];   // pieces before pool p, of one row
   int count;
 };
 
-// One warp per group, lane l its children l and l + 32; sets of beams are 64-bit masks.
-__global__ void __launch_bounds__(kPlanThreads)
-    reorder_plan_kernel(const int32_t* __restrict__ slots, const int32_t* __restrict__ parents,
-                        int32_t* __restrict__ new_slots, int2* __restrict__ copies,
-                        int* __restrict__ n_copies, int G, int K, int rows, unsigned int* status) {
+__global__ void __launch_bounds__(kCopyThreads)
+    reorder_kernel(const __grid_constant__ ReorderPools pools, const int32_t* __restrict__ slots,
+                   const int32_t* __restrict__ parents, int32_t* __restrict__ new_slots, int G,
+                   int K, int rows, unsigned int* status) {
   constexpr unsigned kAll = 0xffffffffu;
+  constexpr int kUnit = kCopyThreads * kCopyVecs;
+  // Per copied source, at K / 2 places a group: its row, where its destinations start and
+  // how many there are. `order` lists the places in use, in the same order in every CTA.
+  __shared__ int src_row[kPlanBeams / 2], src_at[kPlanBeams / 2], src_n[kPlanBeams / 2];
+  __shared__ int dst_row[kPlanBeams], in_group[kPlanBeams], order[kPlanBeams / 2];
+  __shared__ int n_src;
   pdl_wait();
   pdl_trigger();
-  __shared__ int total;
-  if (threadIdx.x == 0) total = 0;
-  __syncthreads();
   const int lane = threadIdx.x & 31;
   const uint64_t beams = K == 64 ? ~0ull : (1ull << K) - 1ull;
-  for (int g = threadIdx.x >> 5; g < G; g += kPlanThreads / 32) {
-    const int32_t* mine = slots + (size_t)g * K;
-    int p[2];
-    uint64_t used = 0, later = 0;
+  const int slice = kPlanBeams / K;  // groups planned at once
+  const bool writes = blockIdx.x == 0;
+  for (int g0 = 0; g0 < G; g0 += slice) {
+    for (int g = g0 + (threadIdx.x >> 5); g < min(G, g0 + slice); g += kCopyThreads / 32) {
+      const int32_t* mine = slots + (size_t)g * K;
+      int p[2], slot[2], own[2];
+      uint64_t used = 0, later = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int j = lane + 32 * i;
-      p[i] = j < K ? parents[(size_t)g * K + j] : -1;
-      const bool ok = p[i] >= 0 && p[i] < K;
-      if (j < K && !ok) flag_device(status, DEV_BAD_INDEX);
-      // A child is a later one if its beam has a child among the lower lanes or lanes
-      // 0-31 of the first round.
-      const unsigned same = __match_any_sync(kAll, ok ? p[i] : -1);
-      const bool again = ok && ((same & ((1u << lane) - 1u)) != 0u || (used >> p[i] & 1ull));
-      later |= (uint64_t)__ballot_sync(kAll, again) << (32 * i);
-      const uint64_t bit = ok ? 1ull << p[i] : 0ull;
-      used |= (uint64_t)__reduce_or_sync(kAll, (unsigned)bit) |
-              ((uint64_t)__reduce_or_sync(kAll, (unsigned)(bit >> 32)) << 32);
-    }
-    const uint64_t dead = beams & ~used;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int j = lane + 32 * i;
-      if (j >= K) continue;
-      int slot = -1;
-      if (p[i] >= 0 && p[i] < K) {
-        const int src = mine[p[i]];
-        slot = src;
-        if (later >> j & 1ull) {
-          uint64_t d = dead;  // as many beams without children as later ones, at least
-          for (int skip = __popcll(later & ((1ull << j) - 1ull)); skip > 0; --skip) d &= d - 1;
-          slot = d != 0 ? mine[__ffsll(d) - 1] : -1;
-          if (src >= 0 && src < rows && slot >= 0 && slot < rows)
-            copies[atomicAdd(&total, 1)] = make_int2(src, slot);
-        }
-        if (src < 0 || src >= rows || slot < 0 || slot >= rows) flag_device(status, DEV_BAD_INDEX);
+      for (int i = 0; i < 2; ++i) {
+        const int j = lane + 32 * i;
+        p[i] = j < K ? parents[(size_t)g * K + j] : -1;
+        own[i] = j < K ? mine[j] : -1;  // beam j's own row
+        const bool ok = p[i] >= 0 && p[i] < K;
+        if (j < K && !ok && writes) flag_device(status, DEV_BAD_INDEX);
+        // A child is a later one if its beam has a child among the lower lanes or, in the
+        // second round, among the first 32.
+        const unsigned same = __match_any_sync(kAll, ok ? p[i] : -1);
+        const bool again = ok && ((same & ((1u << lane) - 1u)) != 0u || (used >> p[i] & 1ull));
+        later |= (uint64_t)__ballot_sync(kAll, again) << (32 * i);
+        const uint64_t bit = ok ? 1ull << p[i] : 0ull;
+        used |= (uint64_t)__reduce_or_sync(kAll, (unsigned)bit) |
+                ((uint64_t)__reduce_or_sync(kAll, (unsigned)(bit >> 32)) << 32);
       }
-      new_slots[(size_t)g * K + j] = slot;
+      const uint64_t dead = beams & ~used;
+      const auto row_of = [&](int b) {  // all lanes; b in [0, 64)
+        const int lo = __shfl_sync(kAll, own[0], b & 31), hi = __shfl_sync(kAll, own[1], b & 31);
+        return b < 32 ? lo : hi;
+      };
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = lane + 32 * i;
+        const bool ok = p[i] >= 0 && p[i] < K;
+        const bool copy = later >> j & 1ull;
+        const int src = row_of(ok ? p[i] : 0);
+        uint64_t d = dead;  // as many beams without children as later children, at least
+        if (copy)
+          for (int skip = __popcll(later & ((1ull << j) - 1ull)); skip > 0; --skip) d &= d - 1;
+        const int to = row_of(copy && d != 0 ? __ffsll(d) - 1 : 0);
+        slot[i] = !ok ? -1 : copy ? to : src;
+        const bool bad = ok && (src < 0 || src >= rows || slot[i] < 0 || slot[i] >= rows);
+        if (bad && writes) flag_device(status, DEV_BAD_INDEX);
+        if (j < K && writes) new_slots[(size_t)g * K + j] = slot[i];
+        if (!copy || bad) slot[i] = -1;
+      }
+      // Beams with copies, one after the other.
+      int at = (g - g0) * (K / 2), to = (g - g0) * K;
+      for (uint64_t left = used; left != 0; left &= left - 1) {
+        const int b = __ffsll(left) - 1;
+        const uint64_t mine_b =
+            (uint64_t)__ballot_sync(kAll, slot[0] >= 0 && p[0] == b) |
+            ((uint64_t)__ballot_sync(kAll, slot[1] >= 0 && p[1] == b) << 32);
+        if (mine_b == 0) continue;
+        const int row = row_of(b), cnt = __popcll(mine_b);
+        if (lane == 0) {
+          src_row[at] = row;
+          src_at[at] = to;
+          src_n[at] = cnt;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = lane + 32 * i;
+          if (mine_b >> j & 1ull) dst_row[to + __popcll(mine_b & ((1ull << j) - 1ull))] = slot[i];
+        }
+        ++at;
+        to += cnt;
+      }
+      if (lane == 0) in_group[g - g0] = at - (g - g0) * (K / 2);
     }
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) *n_copies = total;
-}
-
-__global__ void __launch_bounds__(kCopyThreads)
-    reorder_copy_kernel(const __grid_constant__ ReorderPools pools, const int2* __restrict__ copies,
-                        const int* __restrict__ n_copies, int rows) {
-  pdl_wait();
-  pdl_trigger();
-  const int n = *n_copies;
-  const long long units = pools.first[pools.count] * n;
-  constexpr int kUnit = kCopyThreads * kCopyVecs;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const long long part = u / n;  // consecutive units: the copies of one place
-    const int2 cp = copies[u - part * n];
-    int p = 0;
-    while (p + 1 < pools.count && part >= pools.first[p + 1]) ++p;
-    const long long per_row = (pools.chunks[p] + kUnit - 1) / kUnit;
-    const long long at = part - pools.first[p];
-    const int layer = (int)(at / per_row);
-    const long long c0 = (at - layer * per_row) * kUnit + threadIdx.x;
-    uint4* base = reinterpret_cast<uint4*>(pools.base[p]) + (size_t)layer * rows * pools.chunks[p];
-    const uint4* src = base + (size_t)cp.x * pools.chunks[p];
-    uint4* dst = base + (size_t)cp.y * pools.chunks[p];
-    uint4 v[kCopyVecs];
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      int before = 0;
+      for (int x = 0; x < min(slice, G - g0); x += 32) {
+        const int cnt = x + lane < min(slice, G - g0) ? in_group[x + lane] : 0;
+        int incl = cnt;
 #pragma unroll
-    for (int i = 0; i < kCopyVecs; ++i)
-      if (c0 + i * kCopyThreads < pools.chunks[p]) v[i] = src[c0 + i * kCopyThreads];
+        for (int off = 1; off < 32; off <<= 1) {
+          const int y = __shfl_up_sync(kAll, incl, off);
+          if (lane >= off) incl += y;
+        }
+        for (int i = 0; i < cnt; ++i) order[before + incl - cnt + i] = (x + lane) * (K / 2) + i;
+        before += __shfl_sync(kAll, incl, 31);
+      }
+      if (lane == 0) n_src = before;
+    }
+    __syncthreads();
+    const int n = n_src;
+    const long long units = pools.first[pools.count] * n;
+    for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+      const long long part = u / n;
+      const int i = order[u - part * n];
+      int p = 0;
+      while (p + 1 < pools.count && part >= pools.first[p + 1]) ++p;
+      const long long per_row = (pools.chunks[p] + kUnit - 1) / kUnit;
+      const long long at = part - pools.first[p];
+      const int layer = (int)(at / per_row);
+      const long long c0 = (at - layer * per_row) * kUnit + threadIdx.x;
+      uint4* base = reinterpret_cast<uint4*>(pools.base[p]) + (size_t)layer * rows * pools.chunks[p];
+      const uint4* src = base + (size_t)src_row[i] * pools.chunks[p];
+      uint4 v[kCopyVecs];
 #pragma unroll
-    for (int i = 0; i < kCopyVecs; ++i)
-      if (c0 + i * kCopyThreads < pools.chunks[p]) dst[c0 + i * kCopyThreads] = v[i];
+      for (int x = 0; x < kCopyVecs; ++x)
+        if (c0 + x * kCopyThreads < pools.chunks[p]) v[x] = __ldcs(src + c0 + x * kCopyThreads);
+      for (int d = 0; d < src_n[i]; ++d) {
+        uint4* dst = base + (size_t)dst_row[src_at[i] + d] * pools.chunks[p];
+#pragma unroll
+        for (int x = 0; x < kCopyVecs; ++x)
+          if (c0 + x * kCopyThreads < pools.chunks[p]) __stcs(dst + c0 + x * kCopyThreads, v[x]);
+      }
+    }
+    __syncthreads();
   }
 }
 
 template <typename T>
-cudaError_t launch_select(SelectArgs a, int vecs, cudaStream_t s) {
-  const dim3 grid(a.chunks, a.G * a.K);
-  cudaError_t err = launch_pdl(vecs == 2 ? scan_kernel<T, 2> : scan_kernel<T, 8>, grid,
-                               dim3(kScanThreads), 0, s, a);
+cudaError_t launch_select(const SelectArgs& a, cudaStream_t s) {
+  const cudaError_t err =
+      launch_pdl(scan_kernel<T>, dim3(a.segs, a.G * a.K), dim3(kScanThreads), 0, s, a);
   if (err != cudaSuccess) return err;
   return launch_pdl(merge_kernel<T>, dim3(a.G), dim3(kMergeThreads), 0, s, a);
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// The parts of the workspace: stats, counts, floors, kept logits, kept tokens.
-size_t select_layout(long long segs, size_t* at) {
+// The parts of the workspace: stats, floors, candidates.
+size_t select_layout(long long segs, int n, size_t* at) {
+  const size_t sizes[3] = {sizeof(float2) * (size_t)segs, sizeof(float) * (size_t)segs,
+                           sizeof(uint2) * (size_t)segs * (n + 1)};
   size_t o = 0;
-  const size_t sizes[5] = {sizeof(float2) * (size_t)segs, sizeof(int) * (size_t)segs,
-                           sizeof(float) * (size_t)segs, sizeof(float) * (size_t)segs * kSegment,
-                           sizeof(int32_t) * (size_t)segs * kSegment};
-  for (int i = 0; i < 5; ++i) {
+  for (int i = 0; i < 3; ++i) {
     if (at != nullptr) at[i] = o;
     o += round256(sizes[i]);
   }
@@ -624,14 +895,13 @@ size_t select_layout(long long segs, size_t* at) {
 }  // namespace
 }  // namespace sc
 
-extern "C" size_t sc_beam_select_workspace(int groups, int beams, int vocab, int logits_fp32) {
-  if (groups <= 0 || beams <= 0 || vocab <= 0) return 0;
+extern "C" size_t sc_beam_select_workspace(int groups, int beams, int vocab, int n,
+                                           int logits_fp32) {
+  if (groups <= 0 || beams <= 0 || vocab <= 0 || n <= 0 || n > sc::kMaxSelect) return 0;
   const long long rows = (long long)groups * beams;
-  const int vecs = logits_fp32 ? sc::select_vecs<float>(rows, vocab)
-                               : sc::select_vecs<uint16_t>(rows, vocab);
-  const int chunks = logits_fp32 ? sc::chunk_count<float>(vocab, vecs)
-                                 : sc::chunk_count<uint16_t>(vocab, vecs);
-  return sc::select_layout(rows * chunks, nullptr);
+  const sc::Segments seg = logits_fp32 ? sc::select_segments<float>(rows, vocab)
+                                       : sc::select_segments<uint16_t>(rows, vocab);
+  return sc::select_layout(rows * seg.count, n, nullptr);
 }
 
 extern "C" int sc_beam_select(const void* logits, int logits_fp32, int64_t row_stride,
@@ -659,27 +929,25 @@ extern "C" int sc_beam_select(const void* logits, int logits_fp32, int64_t row_s
   SC_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (logits_fp32 ? 4 : 2) == 0 &&
                  reinterpret_cast<uintptr_t>(workspace) % 256 == 0,
              SC_ERR_INVALID, "%s: misaligned logits or workspace (256 bytes)", name);
-  const size_t need = sc_beam_select_workspace(groups, beams, vocab, logits_fp32);
+  const size_t need = sc_beam_select_workspace(groups, beams, vocab, n, logits_fp32);
   SC_REQUIRE(workspace_bytes >= need, SC_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", name,
              workspace_bytes, need);
   const long long rows = (long long)groups * beams;
-  const int vecs = logits_fp32 ? sc::select_vecs<float>(rows, vocab)
-                               : sc::select_vecs<uint16_t>(rows, vocab);
-  sc::SelectArgs a;
-  a.chunks = logits_fp32 ? sc::chunk_count<float>(vocab, vecs)
-                         : sc::chunk_count<uint16_t>(vocab, vecs);
-  size_t at[5];
-  sc::select_layout(rows * a.chunks, at);
+  const sc::Segments seg = logits_fp32 ? sc::select_segments<float>(rows, vocab)
+                                       : sc::select_segments<uint16_t>(rows, vocab);
+  size_t at[3];
+  sc::select_layout(rows * seg.count, n, at);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  sc::SelectArgs a;
+  a.segs = seg.count;
+  a.seg_blocks = seg.blocks;
   a.logits = logits;
   a.row_stride = row_stride;
   a.scores = scores;
   a.finished = finished;
   a.stats = reinterpret_cast<float2*>(ws + at[0]);
-  a.counts = reinterpret_cast<int*>(ws + at[1]);
-  a.floors = reinterpret_cast<float*>(ws + at[2]);
-  a.kept_x = reinterpret_cast<float*>(ws + at[3]);
-  a.kept_v = reinterpret_cast<int32_t*>(ws + at[4]);
+  a.floors = reinterpret_cast<float*>(ws + at[1]);
+  a.kept = reinterpret_cast<uint2*>(ws + at[2]);
   a.out_scores = out_scores;
   a.parents = parents;
   a.tokens = tokens;
@@ -689,8 +957,8 @@ extern "C" int sc_beam_select(const void* logits, int logits_fp32, int64_t row_s
   a.n = n;
   a.pad = pad_token;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = logits_fp32 ? sc::launch_select<float>(a, vecs, s)
-                                      : sc::launch_select<uint16_t>(a, vecs, s);
+  const cudaError_t err = logits_fp32 ? sc::launch_select<float>(a, s)
+                                      : sc::launch_select<uint16_t>(a, s);
   if (err != cudaSuccess)
     return sc::set_error(SC_ERR_CUDA, "%s: launch: %s", name, cudaGetErrorString(err));
   return sc::check_launch(name);
@@ -698,20 +966,15 @@ extern "C" int sc_beam_select(const void* logits, int logits_fp32, int64_t row_s
 
 extern "C" int sc_reorder_rows(void* const* pools, const int64_t* row_bytes, const int* layers,
                                int npools, int rows, const int32_t* slots, const int32_t* parents,
-                               int32_t* new_slots, int32_t* copies, int groups, int beams,
-                               void* stream) {
+                               int32_t* new_slots, int groups, int beams, void* stream) {
   const char* name = "sc_reorder_rows";
   SC_REQUIRE(npools >= 0 && npools <= 4 && rows > 0 && groups >= 0 && beams > 0, SC_ERR_INVALID,
              "%s: bad npools=%d rows=%d groups=%d beams=%d", name, npools, rows, groups, beams);
   SC_REQUIRE(beams <= sc::kMaxBeams, SC_ERR_UNSUPPORTED, "%s: %d beams, at most %d", name, beams,
              sc::kMaxBeams);
   if (groups == 0) return SC_OK;
-  SC_REQUIRE(slots && parents && new_slots && copies && (npools == 0 || (pools && row_bytes && layers)),
+  SC_REQUIRE(slots && parents && new_slots && (npools == 0 || (pools && row_bytes && layers)),
              SC_ERR_INVALID, "%s: null pointer", name);
-  SC_REQUIRE((long long)groups * beams <= (1 << 20), SC_ERR_UNSUPPORTED, "%s: %lld beams in all",
-             name, (long long)groups * beams);
-  SC_REQUIRE(reinterpret_cast<uintptr_t>(copies) % 8 == 0, SC_ERR_INVALID,
-             "%s: copies must be 8-byte aligned", name);
   sc::ReorderPools p = {};
   p.count = npools;
   for (int i = 0; i < npools; ++i) {
@@ -720,20 +983,15 @@ extern "C" int sc_reorder_rows(void* const* pools, const int64_t* row_bytes, con
                SC_ERR_INVALID, "%s: pool %d: 16-byte aligned rows of a multiple of 16 bytes", name, i);
     p.base[i] = static_cast<uint8_t*>(pools[i]);
     p.chunks[i] = row_bytes[i] / 16;
-    p.layers[i] = layers[i];
     const long long unit = sc::kCopyThreads * sc::kCopyVecs;
     p.first[i + 1] = p.first[i] + layers[i] * ((p.chunks[i] + unit - 1) / unit);
   }
-  // The plan's scratch: the copy count, then the (source, destination) pairs.
-  int* n_copies = reinterpret_cast<int*>(copies);
-  int2* pairs = reinterpret_cast<int2*>(copies + 2);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t err = sc::launch_pdl(sc::reorder_plan_kernel, dim3(1), dim3(sc::kPlanThreads), 0, s,
-                                   slots, parents, new_slots, pairs, n_copies, groups, beams, rows,
-                                   sc::device_status_word());
-  if (err == cudaSuccess && npools > 0 && p.first[npools] > 0)
-    err = sc::launch_pdl(sc::reorder_copy_kernel, dim3(148 * 8), dim3(sc::kCopyThreads), 0, s, p,
-                         static_cast<const int2*>(pairs), static_cast<const int*>(n_copies), rows);
+  // Eight CTAs an SM; fewer where there are fewer pieces to copy than that.
+  const long long most = p.first[npools] * groups * (beams / 2);
+  const int ctas = (int)(most < 1 ? 1 : most > 148 * 8 ? 148 * 8 : most);
+  const cudaError_t err = sc::launch_pdl(sc::reorder_kernel, dim3(ctas), dim3(sc::kCopyThreads), 0,
+                                         static_cast<cudaStream_t>(stream), p, slots, parents,
+                                         new_slots, groups, beams, rows, sc::device_status_word());
   if (err != cudaSuccess)
     return sc::set_error(SC_ERR_CUDA, "%s: launch: %s", name, cudaGetErrorString(err));
   return sc::check_launch(name);

@@ -17,9 +17,12 @@
 //
 // B200 mapping. HBM-bound: each value is read and written once. A CTA makes the
 // (cos, sin) table of its tokens in shared memory, then its warps walk the tokens'
-// head rows (q, k, v); D / 8 lanes hold a row, 8 values each, so a row moves as
-// 16-byte accesses, the norm is a shuffle sum and the partner of a pair is a
-// shuffle away (R / 2 is a multiple of 8).
+// head rows (q, k, v). D / 8 lanes hold a row, 8 values each as two 4-value pieces: a
+// lane of the rotary part holds both halves of four pairs, so that a turn needs no
+// exchange, and the norm is a shuffle sum. Two rows are loaded before the first is
+// computed; the norm's weights stay in registers.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace sc {
@@ -40,37 +43,35 @@ struct RotaryArgs {
   const int64_t* slots;
   long long num_pages;
   float eps;
-  int ntok, Hq, Hkv, half, axes, P;
+  int ntok, Hq, Hkv, half, axes, P, page_shift;
   unsigned int* status;
 };
 
-// 8 consecutive bf16 of a row; without kVec the address has 2-byte alignment only.
+// 4 consecutive bf16 of a row; without kVec the address has 2-byte alignment only.
 template <bool kVec>
-__device__ __forceinline__ uint4 load8(const uint16_t* p) {
-  if constexpr (kVec) {
-    return *reinterpret_cast<const uint4*>(p);
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
+__device__ __forceinline__ uint2 load4(const uint16_t* p) {
+  if constexpr (kVec)
+    return *reinterpret_cast<const uint2*>(p);
+  else
+    return make_uint2((uint32_t)p[0] | ((uint32_t)p[1] << 16),
+                      (uint32_t)p[2] | ((uint32_t)p[3] << 16));
 }
 
-__device__ __forceinline__ void unpack8(const uint4& u, float* x) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = bf16_lo(w[i]);
-    x[2 * i + 1] = bf16_hi(w[i]);
-  }
+__device__ __forceinline__ void unpack4(const uint2& u, float* x) {
+  x[0] = bf16_lo(u.x);
+  x[1] = bf16_hi(u.x);
+  x[2] = bf16_lo(u.y);
+  x[3] = bf16_hi(u.y);
 }
 
 template <int D, bool kVec>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a, int tokens) {
   constexpr int kLanes = D / 8;              // lanes of one row
   constexpr int kRows = 32 / kLanes;         // rows of one warp
-  extern __shared__ float2 table[];          // [tokens][half] (cos, sin)
+  constexpr int kStep = kRotThreads / 32 * kRows;
+  constexpr int kAhead = 2;                  // rows in flight per lane
+  extern __shared__ float4 table4[];         // [tokens][half] (cos, sin)
+  float2* table = reinterpret_cast<float2*>(table4);
   pdl_wait();
   pdl_trigger();
   const int t0 = blockIdx.x * tokens;
@@ -83,78 +84,122 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a,
     sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
     table[i] = make_float2(c, s);
   }
-  __syncthreads();
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = lane % kLanes;               // this lane's 16-byte chunk of its row
-  const int heads = a.Hq + 2 * a.Hkv;
-  const int nrows = nt * heads;
-  const int step = kRotThreads / 32 * kRows * gridDim.y;
-  const int hc = a.half / 8;                 // chunks of half the rotary dims
-  // The partner of a rotary chunk holds the other halves of its pairs.
-  const int partner = (c < hc ? c + hc : (c < 2 * hc ? c - hc : c)) + (lane - c);
-  for (int r0 = (blockIdx.y * (kRotThreads / 32) + warp) * kRows; r0 < nrows; r0 += step) {
-    const int r = r0 + lane / kLanes;
-    const bool live = r < nrows;
-    const int t = live ? r / heads : 0;
-    const int h = live ? r - t * heads : 0;
-    const long long tok = t0 + t;
-    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
-    const int kvh = is_q ? 0 : (is_v ? h - a.Hq - a.Hkv : h - a.Hq);
-    uint16_t* dst = nullptr;
-    const uint16_t* src;
-    if (is_q) {
-      src = a.q + tok * a.q_tok + h * a.q_head;
-      dst = a.q_out + ((size_t)tok * a.Hq + h) * D + 8 * c;
-    } else {
-      src = is_v ? a.v + tok * a.v_tok + kvh * a.v_head : a.k + tok * a.k_tok + kvh * a.k_head;
-      if (a.pool != nullptr) {
-        const int64_t slot = a.slots[tok];
-        const int64_t page = slot / a.P;
-        if (slot >= 0 && page < a.num_pages) {
-          const int off = (int)(slot - page * a.P);
-          dst = a.pool + ((((size_t)page * a.Hkv + kvh) * 2 + is_v) * a.P + off) * D +
-                8 * (c ^ (off & 7));
-        } else if (slot >= 0 && c == 0 && live) {
-          flag_device(a.status, DEV_BAD_INDEX);
+  const int c = lane % kLanes;
+  // This lane's pieces: of the rotary part the c-th of each half, of the rest two
+  // neighbours. lo / hi are their first elements.
+  const int turning = a.half / 4;            // lanes of the rotary part
+  const bool turns = c < turning;
+  const int lo = turns ? 4 * c : 8 * c;  // 2 half + 8 (c - half / 4)
+  const int hi = turns ? lo + a.half : lo + 4;
+
+  // The rows (token, head) of one operand, kStep * gridDim.y apart for this lane's; kKind:
+  // 0 q, 1 k, 2 v. All lanes of a warp go around alike: the shuffles want the whole warp.
+  const auto walk = [&](auto kind, int nheads, int skew, const uint16_t* in, long long in_tok,
+                        long long in_head, const float* w, bool norm) {
+    constexpr int kKind = decltype(kind)::value;
+    const int step = kStep * gridDim.y;
+    // Operands start on different warps, so that a few heads do not all fall on the first.
+    int h = ((blockIdx.y * (kRotThreads / 32) + warp) * kRows + lane / kLanes + step - skew) % step;
+    int t = 0;
+    const auto settle = [&]() {
+      while (h >= nheads) {
+        h -= nheads;
+        ++t;
+      }
+    };
+    settle();
+    while (__any_sync(0xffffffffu, t < nt)) {
+      uint2 u[kAhead][2];
+      uint16_t* dst[kAhead];
+      int tt[kAhead], flip[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        tt[i] = t;
+        flip[i] = 0;
+        dst[i] = nullptr;
+        u[i][0] = u[i][1] = make_uint2(0u, 0u);
+        if (t < nt) {
+          const int tok = t0 + t;
+          if constexpr (kKind == 0) {
+            dst[i] = a.q_out + ((size_t)tok * nheads + h) * D;
+          } else if (a.pool != nullptr) {
+            const int64_t slot = a.slots[tok];
+            const int64_t page = slot >> a.page_shift;
+            if (slot >= 0 && page < a.num_pages) {
+              const int off = (int)slot & (a.P - 1);
+              dst[i] = a.pool + ((((size_t)page * nheads + h) * 2 + (kKind == 2)) * a.P + off) * D;
+              flip[i] = 8 * (off & 7);  // 16-byte chunks move, halves of one stay
+            } else if (slot >= 0 && c == 0) {
+              flag_device(a.status, DEV_BAD_INDEX);
+            }
+          } else if constexpr (kKind == 1) {
+            dst[i] = a.k_out + ((size_t)tok * nheads + h) * D;
+          }
+          if (dst[i] != nullptr) {
+            const uint16_t* src = in + tok * in_tok + h * in_head;
+            u[i][0] = load4<kVec>(src + lo);
+            u[i][1] = load4<kVec>(src + hi);
+          }
         }
-      } else if (!is_v) {
-        dst = a.k_out + ((size_t)tok * a.Hkv + kvh) * D + 8 * c;
+        h += step;
+        settle();
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if constexpr (kKind != 2) {
+          float x[8];
+          unpack4(u[i][0], x);
+          unpack4(u[i][1], x + 4);
+          if (norm) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+#pragma unroll
+            for (int off = kLanes / 2; off >= 1; off >>= 1)
+              sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            const float inv = rsqrtf(sum * (1.f / D) + a.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
+          }
+          if (turns && tt[i] < nt) {
+            const float4* cs = table4 + (tt[i] * a.half + 4 * c) / 2;
+            const float4 p = cs[0], r = cs[1];
+            const float co[4] = {p.x, p.z, r.x, r.z}, si[4] = {p.y, p.w, r.y, r.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y = x[e], z = x[4 + e];
+              x[e] = y * co[e] - z * si[e];
+              x[4 + e] = z * co[e] + y * si[e];
+            }
+          }
+          u[i][0] = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+          u[i][1] = make_uint2(pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+        }
+        if (dst[i] != nullptr) {
+          *reinterpret_cast<uint2*>(dst[i] + (lo ^ flip[i])) = u[i][0];
+          *reinterpret_cast<uint2*>(dst[i] + (hi ^ flip[i])) = u[i][1];
+        }
       }
     }
-    uint4 u = make_uint4(0u, 0u, 0u, 0u);
-    if (live && dst != nullptr) u = load8<kVec>(src + 8 * c);
-    float x[8];
-    unpack8(u, x);
-    const uint16_t* w = is_q ? a.q_weight : a.k_weight;
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-    for (int off = kLanes / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (w != nullptr && !is_v) {
-      const float inv = rsqrtf(sum * (1.f / D) + a.eps);
-      float wf[8];
-      unpack8(*reinterpret_cast<const uint4*>(w + 8 * c), wf);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * wf[i];
-    }
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], partner);
-    if (!is_v && c < 2 * hc) {
-      const float2* cs = table + t * a.half + 8 * (c < hc ? c : c - hc);
-      const float sign = c < hc ? -1.f : 1.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * cs[i].x + sign * (y[i] * cs[i].y);
-    }
-    if (live && dst != nullptr) {
-      if (!is_v)
-        u = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                       pack_bf16x2(x[6], x[7]));
-      *reinterpret_cast<uint4*>(dst) = u;
-    }
-  }
+  };
+  float w[8];
+  const auto weights = [&](const uint16_t* p) {
+    if (p == nullptr) return;
+    unpack4(*reinterpret_cast<const uint2*>(p + lo), w);
+    unpack4(*reinterpret_cast<const uint2*>(p + hi), w + 4);
+  };
+  weights(a.q_weight);
+  __syncthreads();
+  walk(std::integral_constant<int, 0>{}, a.Hq, 0, a.q, a.q_tok, a.q_head, w, a.q_weight != nullptr);
+  weights(a.k_weight);
+  const int step = kStep * gridDim.y;
+  walk(std::integral_constant<int, 1>{}, a.Hkv, nt * a.Hq % step, a.k, a.k_tok, a.k_head, w,
+       a.k_weight != nullptr);
+  if (a.pool != nullptr)
+    walk(std::integral_constant<int, 2>{}, a.Hkv, nt * (a.Hq + a.Hkv) % step, a.v, a.v_tok, a.v_head,
+         w, false);
 }
 
 template <int D>
@@ -234,6 +279,7 @@ extern "C" int sc_rotary_append(const sc_bf16* q, const sc_bf16* k, const sc_bf1
   a.half = rotary_dim / 2;
   a.axes = axes;
   a.P = kv_pool != nullptr ? P : 16;
+  a.page_shift = a.P == 8 ? 3 : a.P == 16 ? 4 : 5;
   a.status = sc::device_status_word();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t err = D == 64    ? sc::launch_rotary<64>(a, vec, s)

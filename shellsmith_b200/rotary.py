@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _capi, paged
-from ._torch import ptr, require_cuda, stream_of
+from ._torch import require_cuda, stream_of
 
 
 class RotaryPlan:
@@ -56,6 +56,8 @@ class RotaryPlan:
                                  device=device)
         self.inv_freq = torch.tensor(inv_freq, dtype=torch.float64)
         self.turns = (self.inv_freq / (2 * math.pi)).to(device)  # whole turns per position
+        self.device_index = self.turns.get_device()
+        self.turns_ptr, self.axis_ptr = self.turns.data_ptr(), self.axis.data_ptr()
 
 
 def axis_of_pairs(sections, interleaved: bool) -> list:
@@ -66,47 +68,54 @@ def axis_of_pairs(sections, interleaved: bool) -> list:
     return [i % count if i < count * sections[i % count] else 0 for i in range(half)]
 
 
-def _operand(name: str, t: torch.Tensor, plan: RotaryPlan) -> None:
+_append = _capi.bind("sc_rotary_append")
+_Strides = ctypes.c_int64 * 6
+
+
+def _operand(name: str, t: torch.Tensor, dim: int) -> tuple:
+    """Shape and strides of a [ntok, heads, D] bf16 operand."""
+    if type(t) is torch.Tensor and t.is_cuda and t.dtype is torch.bfloat16 and t.dim() == 3:
+        shape, stride = t.shape, t.stride()
+        if shape[2] == dim and (stride[2] == 1 or not t.numel()):
+            return shape, stride
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (the product path has no CPU fallback)")
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} must be torch.bfloat16, got {t.dtype}")
-    if t.dim() != 3 or t.shape[2] != plan.head_dim:
-        raise ValueError(f"{name} must be [ntok, heads, {plan.head_dim}], got {tuple(t.shape)}")
-    if t.stride(2) != 1 and t.numel():
-        raise ValueError(f"{name} must be contiguous along the head dimension")
+    if t.dim() != 3 or t.shape[2] != dim:
+        raise ValueError(f"{name} must be [ntok, heads, {dim}], got {tuple(t.shape)}")
+    raise ValueError(f"{name} must be contiguous along the head dimension")
 
 
-def _run(q, k, v, positions, plan, q_weight, k_weight, eps, q_out, k_out, pool, slots) -> None:
-    _operand("q", q, plan)
-    _operand("k", k, plan)
-    ntok, hq, dim = q.shape
-    hkv = k.shape[1]
-    if k.shape[0] != ntok:
+def _weight(name: str, w: torch.Tensor | None, dim: int) -> int | None:
+    if w is None:
+        return None
+    require_cuda(name, w, torch.bfloat16, 1)
+    if w.shape[0] != dim:
+        raise ValueError(f"{name} must have {dim} entries")
+    return w.data_ptr()
+
+
+def _run(q, k, v, k_shape, strides, positions, plan, q_weight, k_weight, eps, q_out, k_out, pool,
+         slots, page, pages) -> None:
+    dim, ntok = plan.head_dim, q.shape[0]
+    if k_shape[0] != ntok:
         raise ValueError("rotary: q and k must have the same tokens")
-    if positions.dim() == 1:
-        positions = positions[None]
-    if (positions.dtype != torch.int32 or not positions.is_cuda
-            or tuple(positions.shape) != (plan.axes, ntok)
-            or (ntok > 1 and positions.stride(1) != 1)):
+    shape, pos_stride = positions.shape, positions.stride()
+    if len(shape) == 1:
+        shape, pos_stride = (1, *shape), (0, *pos_stride)
+    if (positions.dtype is not torch.int32 or not positions.is_cuda or len(shape) != 2
+            or shape[0] != plan.axes or shape[1] != ntok or (ntok > 1 and pos_stride[1] != 1)):
         raise ValueError(f"positions must be CUDA int32 [{plan.axes}, {ntok}] (one row per axis), "
                          f"got {positions.dtype} {tuple(positions.shape)}")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            require_cuda(name, w, torch.bfloat16, 1)
-            if w.shape[0] != dim:
-                raise ValueError(f"{name} must have {dim} entries")
-    if plan.turns.device != q.device:
+    if plan.device_index != q.get_device():
         raise ValueError(f"the plan is on {plan.turns.device}, q on {q.device}")
-    pages, page = (0, 0) if pool is None else (pool.shape[0], pool.shape[3])
-    vs = (0, 0) if v is None else v.stride()
-    strides = (ctypes.c_int64 * 6)(q.stride(0), q.stride(1), k.stride(0), k.stride(1), vs[0], vs[1])
-    _capi.call("sc_rotary_append", ptr(q), ptr(k), ptr(v), strides, ptr(positions),
-               positions.stride(0), plan.axes, ptr(plan.turns), ptr(plan.axis), ptr(q_weight),
-               ptr(k_weight), float(eps), ptr(q_out), ptr(k_out), ptr(pool), ptr(slots), ntok, hq,
-               hkv, dim, plan.rotary_dim, page, pages, stream_of(q))
+    _append(q.data_ptr(), k.data_ptr(), v, _Strides(*strides), positions.data_ptr(), pos_stride[0],
+            plan.axes, plan.turns_ptr, plan.axis_ptr, _weight("q_weight", q_weight, dim),
+            _weight("k_weight", k_weight, dim), eps, q_out.data_ptr(), k_out, pool, slots, ntok,
+            q.shape[1], k_shape[1], dim, plan.rotary_dim, page, pages, stream_of(q))
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan: RotaryPlan, *,
@@ -117,11 +126,11 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan: Rota
     positions: int32 [axes, ntok] (or [ntok] for one axis). q and k may be strided
     views with a contiguous last dimension. Returns new contiguous (q, k).
     """
-    _operand("q", q, plan)
-    _operand("k", k, plan)
-    q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    k_out = torch.empty(k.shape, dtype=torch.bfloat16, device=k.device)
-    _run(q, k, None, positions, plan, q_weight, k_weight, eps, q_out, k_out, None, None)
+    q_shape, qs = _operand("q", q, plan.head_dim)
+    k_shape, ks = _operand("k", k, plan.head_dim)
+    q_out, k_out = q.new_empty(q_shape), k.new_empty(k_shape)
+    _run(q, k, None, k_shape, (qs[0], qs[1], ks[0], ks[1], 0, 0), positions, plan, q_weight,
+         k_weight, eps, q_out, k_out.data_ptr(), None, None, 0, 0)
     return q_out, k_out
 
 
@@ -135,22 +144,26 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     its q is still turned). An 8-bit pool takes the turned k from a scratch tensor
     through its own append kernel (two launches).
     """
-    _operand("v", v, plan)
-    if v.shape != k.shape:
+    q_shape, qs = _operand("q", q, plan.head_dim)
+    k_shape, ks = _operand("k", k, plan.head_dim)
+    v_shape, vs = _operand("v", v, plan.head_dim)
+    if v_shape != k_shape:
         raise ValueError("rotary_append: k and v must have the same shape")
-    num_pages, hkv, page, dim = paged._pool_dims(kv_pool)
+    pages, hkv, page, dim = paged._pool_dims(kv_pool)
     require_cuda("slot_mapping", slot_mapping, torch.int64, 1, align=8)
-    if k.shape[1:] != (hkv, dim) or slot_mapping.shape[0] != k.shape[0]:
+    if k_shape[1] != hkv or k_shape[2] != dim or slot_mapping.shape[0] != k_shape[0]:
         raise ValueError("rotary_append: k/v must be [ntok, Hkv, D] with one slot per token")
-    if kv_pool.dtype == torch.uint8:
+    if kv_pool.dtype is torch.uint8:
         q_out, k_out = rotary(q, k, positions, plan, q_weight=q_weight, k_weight=k_weight, eps=eps)
         paged.kv_append(k_out, v.contiguous(), kv_pool, slot_mapping)
         return q_out if out is None else out.copy_(q_out)
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty(q_shape)
     else:
         require_cuda("out", out, torch.bfloat16, 3)
-        if out.shape != q.shape:
+        if out.shape != q_shape:
             raise ValueError("rotary_append: out must have q's shape")
-    _run(q, k, v, positions, plan, q_weight, k_weight, eps, out, None, kv_pool, slot_mapping)
+    _run(q, k, v.data_ptr(), k_shape, (qs[0], qs[1], ks[0], ks[1], vs[0], vs[1]), positions, plan,
+         q_weight, k_weight, eps, out, None, kv_pool.data_ptr(), slot_mapping.data_ptr(), page,
+         pages)
     return out
