@@ -52,31 +52,34 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, *,
         raise ValueError("beam_select: logits must be a [groups, beams, vocab] tensor")
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor (the product path has no CPU fallback)")
-    if logits.dtype not in (torch.bfloat16, torch.float32):
+    fp32 = logits.dtype is torch.float32
+    if not fp32 and logits.dtype is not torch.bfloat16:
         raise TypeError(f"logits must be bfloat16 or float32, got {logits.dtype}")
     groups, beams, vocab = logits.shape
-    if not (logits.is_contiguous() or groups == 0
-            or (logits.stride(2) == 1 and logits.stride(1) >= vocab
-                and (groups == 1 or logits.stride(0) == beams * logits.stride(1)))):
-        raise ValueError("beam_select: logits need a contiguous vocabulary and evenly spaced rows")
+    if beams < 1 or vocab < 1:
+        raise ValueError("beam_select: at least one beam and one token")
+    stride = vocab
+    if not logits.is_contiguous() and groups:
+        across, stride, step = logits.stride()
+        if beams == 1:
+            stride = across if groups > 1 else vocab
+        if (step != 1 and vocab > 1) or stride < vocab or (groups > 1 and across != beams * stride):
+            raise ValueError(
+                "beam_select: logits need a contiguous vocabulary and evenly spaced rows")
     require_cuda("scores", scores, torch.float32, 2, align=4)
-    if tuple(scores.shape) != (groups, beams):
+    if scores.shape != (groups, beams):
         raise ValueError(f"scores must be [{groups}, {beams}], got {tuple(scores.shape)}")
     if finished is not None:
         require_cuda("finished", finished, torch.bool, 2, align=1)
-        if tuple(finished.shape) != (groups, beams):
+        if finished.shape != (groups, beams):
             raise ValueError(f"finished must be [{groups}, {beams}], got {tuple(finished.shape)}")
-    if beams < 1 or vocab < 1:
-        raise ValueError("beam_select: at least one beam and one token")
-    fp32 = int(logits.dtype == torch.float32)
-    need = _workspace(groups, beams, vocab, n, fp32)
-    work = torch.empty(need, dtype=torch.uint8, device=logits.device)
-    best = scores.new_empty((groups, n))
-    parents, tokens = torch.empty((2, groups, n), dtype=torch.int32, device=logits.device).unbind(0)
-    stride = logits.stride(1) if beams > 1 else (logits.stride(0) if groups > 1 else vocab)
-    _select(logits.data_ptr(), fp32, max(stride, vocab), scores.data_ptr(), ptr(finished),
-            pad_token, best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), work.data_ptr(), need,
-            groups, beams, vocab, n, stream_of(logits))
+    need = _workspace(groups, beams, vocab, n, int(fp32))
+    work = scores.new_empty(need // 4)
+    best, parents, tokens = scores.new_empty((3, groups, n)).unbind(0)
+    parents, tokens = parents.view(torch.int32), tokens.view(torch.int32)
+    _select(logits.data_ptr(), fp32, stride, scores.data_ptr(), ptr(finished), pad_token,
+            best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), work.data_ptr(), need, groups,
+            beams, vocab, n, stream_of(logits))
     return best, parents, tokens
 
 

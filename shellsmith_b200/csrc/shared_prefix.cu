@@ -478,7 +478,7 @@ constexpr int kTailWarps = 2;
 constexpr int kTailStages = 3;
 constexpr int kTailHeads = 8;        // query heads of a unit
 constexpr int kTailMaxPages = 32;    // pages of a unit: a lane holds the id of one
-constexpr int kSlabRows = 1024;      // rows a warp searches for its unit
+constexpr int kSlabRows = 1024;      // rows whose units one counter hands out
 
 struct TailArgs {
   const uint16_t *q, *kv_pool;
@@ -514,24 +514,49 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
   uint8_t* stage = smem + warp * kTailStages * STAGE;
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kTailWarps * kTailStages * STAGE) +
                   warp * kTailStages;
+  int* chunks_to = reinterpret_cast<int*>(  // chunks of the slab's rows up to 32 i + 31
+      smem + kTailWarps * kTailStages * (STAGE + sizeof(uint64_t)));
   pdl_trigger();
-  if (lane == 0) {
-    for (int i = 0; i < kTailStages; ++i) mbar_init(&bar[i], 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
   const int slab = blockIdx.y, row0 = slab * kSlabRows;
   const int rows = min(kSlabRows, a.B - row0);
   const int groups = a.Hkv * a.HG;
-
-  struct Unit {
-    int b, kvh, head0, heads, split, n, tokens;  // n pages; tokens of them count
-    int page;                                    // lane i: the id of page i
-  };
   const auto take = [&]() {
     int t = 0;
     if (lane == 0) t = atomicAdd(a.counters + slab, 1);
     return t;
+  };
+  const int t_first = take();
+  if (lane == 0) {
+    for (int i = 0; i < kTailStages; ++i) mbar_init(&bar[i], 1);
+    fence_mbar_init();
+  }
+  const auto own_of = [&](int r) {
+    return r < rows ? own_pages(a.ctx_len[row0 + r], a.first_page[row0 + r], a.max_pages)
+                    : OwnPages{0, 0, 0};
+  };
+  const auto chunks_of = [&](const OwnPages& o) {
+    return min((o.pages + a.pages_per_split - 1) / a.pages_per_split, a.num_splits);
+  };
+#pragma unroll 4
+  for (int i = warp; 32 * i < rows; i += kTailWarps) {
+    const int sum = (int)__reduce_add_sync(kAll, (unsigned)chunks_of(own_of(32 * i + lane)));
+    if (lane == 0) chunks_to[i] = sum;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int incl = 32 * lane < rows ? chunks_to[lane] : 0;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int y = __shfl_up_sync(kAll, incl, off);
+      if (lane >= off) incl += y;
+    }
+    chunks_to[lane] = incl;
+  }
+  __syncthreads();
+
+  struct Unit {
+    int b, kvh, head0, heads, split, n, tokens;  // n pages; tokens of them count
+    int page;                                    // lane i: the id of page i
   };
   // Unit t of the slab: chunk t / groups of the rows' chunks laid end to end. Uniform over
   // the warp; u.n == 0 past the last one.
@@ -540,40 +565,34 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
     t = __shfl_sync(kAll, t, 0);
     const int want = t / groups, hg = t - want * groups;
     u.n = 0;
-    int before = 0;
-    for (int r = 0; r < rows; r += 32) {
-      OwnPages o{0, 0, 0};
-      if (r + lane < rows)
-        o = own_pages(a.ctx_len[row0 + r + lane], a.first_page[row0 + r + lane], a.max_pages);
-      const int mine = min((o.pages + a.pages_per_split - 1) / a.pages_per_split, a.num_splits);
-      int incl = mine;
+    const unsigned past = __ballot_sync(kAll, want < chunks_to[lane]);
+    if (past == 0u) return u;
+    const int block = __ffs(past) - 1;
+    const OwnPages o = own_of(32 * block + lane);
+    const int mine = chunks_of(o);
+    int incl = mine;
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up_sync(kAll, incl, off);
-        if (lane >= off) incl += y;
-      }
-      const unsigned hit = __ballot_sync(kAll, want < before + incl);
-      if (hit != 0u) {
-        const int src = __ffs(hit) - 1;
-        const int chunk = want - before - (__shfl_sync(kAll, incl, src) - __shfl_sync(kAll, mine, src));
-        const int skip = __shfl_sync(kAll, o.skip, src), pages = __shfl_sync(kAll, o.pages, src);
-        const int tokens = __shfl_sync(kAll, o.tokens, src);
-        u.b = row0 + r + src;
-        u.split = chunk;
-        u.n = min(a.pages_per_split, pages - chunk * a.pages_per_split);
-        u.tokens = min(u.n * kPageTok, tokens - chunk * a.pages_per_split * kPageTok);
-        u.page = lane < u.n ? a.block_table[(size_t)u.b * a.max_pages + skip +
-                                            chunk * a.pages_per_split + lane]
-                            : 0;
-        u.kvh = hg / a.HG;
-        u.head0 = u.kvh * a.G + (hg - u.kvh * a.HG) * kTailHeads;
-        u.heads = min(kTailHeads, (u.kvh + 1) * a.G - u.head0);
-        return u;
-      }
-      before += __shfl_sync(kAll, incl, 31);
+    for (int off = 1; off < 32; off <<= 1) {
+      const int y = __shfl_up_sync(kAll, incl, off);
+      if (lane >= off) incl += y;
     }
+    const int left = want - (block > 0 ? chunks_to[block - 1] : 0);
+    const int src = __ffs(__ballot_sync(kAll, left < incl)) - 1;
+    const int chunk = left - (__shfl_sync(kAll, incl, src) - __shfl_sync(kAll, mine, src));
+    const int skip = __shfl_sync(kAll, o.skip, src), pages = __shfl_sync(kAll, o.pages, src);
+    const int tokens = __shfl_sync(kAll, o.tokens, src);
+    const int p0 = chunk * a.pages_per_split;
+    u.b = row0 + 32 * block + src;
+    u.split = chunk;
+    u.n = min(a.pages_per_split, pages - p0);
+    u.tokens = min(u.n * kPageTok, tokens - p0 * kPageTok);
+    u.page = lane < u.n ? a.block_table[(size_t)u.b * a.max_pages + skip + p0 + lane] : 0;
+    u.kvh = hg / a.HG;
+    u.head0 = u.kvh * a.G + (hg - u.kvh * a.HG) * kTailHeads;
+    u.heads = min(kTailHeads, (u.kvh + 1) * a.G - u.head0);
     return u;
   };
+
   int issued = 0, consumed = 0;  // pages of all units, in order through the stages
   const auto issue = [&](const Unit& u, int i) {
     int page = __shfl_sync(kAll, u.page, i);
@@ -599,8 +618,21 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
   ok = __all_sync(kAll, ok);
   Unit cur;
   cur.n = 0;
-  if (ok) cur = resolve(take());
+  if (ok) cur = resolve(t_first);
   int cur_issued = 0;
+  // Q^T as the B operand: b0 = q[n][16kk + 2c .. +1], b1 = q[n][16kk + 8 + 2c .. +1].
+  uint32_t qf[KSTEPS][2];
+  const auto load_q = [&](const Unit& u) {
+    const int n = lane >> 2, c = lane & 3;
+    const bool valid = n < u.heads;
+    const uint16_t* qp = a.q + ((size_t)u.b * a.Hq + u.head0 + (valid ? n : 0)) * D;
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      qf[kk][0] = valid ? *reinterpret_cast<const uint32_t*>(qp + 16 * kk + 2 * c) : 0u;
+      qf[kk][1] = valid ? *reinterpret_cast<const uint32_t*>(qp + 16 * kk + 8 + 2 * c) : 0u;
+    }
+  };
+  if (cur.n > 0) load_q(cur);
   while (ok && cur.n > 0) {
     while (issued - consumed < kTailStages && cur_issued < cur.n) issue(cur, cur_issued++);
     const int t_next = take();
@@ -608,18 +640,6 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
     nxt.n = 0;
     int nxt_issued = 0;
     bool have_next = false;
-    // Q^T as the B operand: b0 = q[n][16kk + 2c .. +1], b1 = q[n][16kk + 8 + 2c .. +1].
-    uint32_t qf[KSTEPS][2];
-    {
-      const int n = lane >> 2, c = lane & 3;
-      const bool valid = n < cur.heads;
-      const uint16_t* qp = a.q + ((size_t)cur.b * a.Hq + cur.head0 + (valid ? n : 0)) * D;
-#pragma unroll
-      for (int kk = 0; kk < KSTEPS; ++kk) {
-        qf[kk][0] = valid ? *reinterpret_cast<const uint32_t*>(qp + 16 * kk + 2 * c) : 0u;
-        qf[kk][1] = valid ? *reinterpret_cast<const uint32_t*>(qp + 16 * kk + 8 + 2 * c) : 0u;
-      }
-    }
     float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F;  // running max of heads 2c, 2c+1 (log2 units)
     float l0 = 0.f, l1 = 0.f;                      // this lane's partial sums
     float o[KSTEPS][4];
@@ -700,6 +720,7 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
       }
     }
     if (!ok) break;
+    if (nxt.n > 0) load_q(nxt);  // arrives while the partial is written
 #pragma unroll
     for (int off = 4; off <= 16; off <<= 1) {
       l0 += __shfl_xor_sync(kAll, l0, off);
@@ -739,8 +760,9 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
 }
 
 // The parts of each (sequence, head) row: those of its prefix, then its own tail's.
-// kWarps warps share a row (a warp's lane holds D / 32 of its columns) and take its
-// parts in turn; a warp holds the parts' weights e^(lse - M), 32 at a time, in its lanes.
+// kWarps warps share a row (a warp's lane holds D / 32 of its columns) and take its parts
+// in turn. Which parts are there follows from the row's context; the loads do not wait for
+// that: every place is read, kAhead of them per warp before anything is known.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeMax = 1024;  // parts of one row
 
@@ -757,68 +779,93 @@ template <int D, int kWarps>
 __global__ void __launch_bounds__(kMergeThreads) merge_parts_kernel(const MergeArgs a) {
   constexpr int kPer = D / 32;                       // columns of a lane
   constexpr int kRows = kMergeThreads / 32 / kWarps; // rows of the CTA
+  constexpr int kAhead = D == 256 ? 3 : 4;
   constexpr unsigned kAll = 0xffffffffu;
   __shared__ float acc_s[kMergeThreads / 32][kWarps > 1 ? D : 1];
   __shared__ float sum_s[kMergeThreads / 32];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp % kWarps;
-  const int row = blockIdx.x * kRows + warp / kWarps;
-  const bool live = row < a.rows;
-  const int b = live ? row / a.Hq : 0;
-  const int ctx = live ? a.ctx_len[b] : 0, first_page = live ? a.first_page[b] : 0;
-  const OwnPages own_pg = own_pages(ctx, first_page, a.max_pages);
-  const int need_pre = (own_pg.skip + a.pre_pps - 1) / a.pre_pps;
-  const int need_own = (own_pg.pages + a.tail_pps - 1) / a.tail_pps;
-  const int n_pre = min(need_pre, a.pre_splits);
-  const int n = n_pre + min(need_own, a.tail_splits);
-  // A context outside the block table, or more pages than the splits cover: clamped.
-  if (lane == 0 && (ctx < 0 || (long long)ctx > (long long)a.max_pages * kPageTok ||
-                    first_page < 0 || first_page > a.max_pages || need_pre > n_pre ||
-                    need_own > n - n_pre))
-    flag_device(a.status, DEV_BAD_INDEX);
+  const int row = min(blockIdx.x * kRows + warp / kWarps, a.rows - 1);  // the last one twice
+  const int total = a.pre_splits + a.tail_splits;
   const size_t pre = (size_t)row * a.pre_splits, own = (size_t)row * a.tail_splits;
   const auto lse_at = [&](int s) {
-    return s < n_pre ? a.pre_lse[pre + s] : a.tail_lse[own + s - n_pre];
+    return s < a.pre_splits ? a.pre_lse[pre + s] : a.tail_lse[own + s - a.pre_splits];
   };
-  // The first 32 parts' lse stay in the lanes; more (many splits) are read again below.
-  const float first = lane < n ? lse_at(lane) : -CUDART_INF_F;
+  const auto load = [&](int s, float* v) {
+    const float* o = s < a.pre_splits ? a.pre_out + (pre + s) * D
+                                      : a.tail_out + (own + s - a.pre_splits) * D;
+    if constexpr (kPer == 2) {
+      const float2 u = reinterpret_cast<const float2*>(o)[lane];
+      v[0] = u.x;
+      v[1] = u.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer / 4; ++i) {
+        const float4 u = reinterpret_cast<const float4*>(o)[lane + 32 * i];
+        v[4 * i] = u.x;
+        v[4 * i + 1] = u.y;
+        v[4 * i + 2] = u.z;
+        v[4 * i + 3] = u.w;
+      }
+    }
+  };
+  float v[kAhead][kPer];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (w + i * kWarps < total) load(w + i * kWarps, v[i]);
+  const float raw = lane < total ? lse_at(lane) : -CUDART_INF_F;
+  const int b = row / a.Hq, ctx = a.ctx_len[b], first_page = a.first_page[b];
+  const OwnPages o = own_pages(ctx, first_page, a.max_pages);
+  const int need_pre = (o.skip + a.pre_pps - 1) / a.pre_pps;
+  const int need_own = (o.pages + a.tail_pps - 1) / a.tail_pps;
+  // A context outside the block table, or more pages than the splits cover: clamped.
+  if (lane == 0 && (ctx < 0 || (long long)ctx > (long long)a.max_pages * kPageTok ||
+                    first_page < 0 || first_page > a.max_pages || need_pre > a.pre_splits ||
+                    need_own > a.tail_splits))
+    flag_device(a.status, DEV_BAD_INDEX);
+  const auto there = [&](int s) {
+    return s < a.pre_splits ? s < need_pre : s - a.pre_splits < need_own && s < total;
+  };
+  const float first = there(lane) ? raw : -CUDART_INF_F;
   float m = first;
-  for (int s = lane + 32; s < n; s += 32) m = fmaxf(m, lse_at(s));
+  for (int s = lane + 32; s < total; s += 32)
+    if (there(s)) m = fmaxf(m, lse_at(s));
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, off));
   float acc[kPer], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  for (int s0 = 0; s0 < n; s0 += 32) {
-    const float ls = s0 == 0 ? first : (s0 + lane < n ? lse_at(s0 + lane) : -CUDART_INF_F);
-    const float e = ls == -CUDART_INF_F ? 0.f : __expf(ls - m);
-    const int cnt = min(32, n - s0);
-#pragma unroll 4
-    for (int s = w; s < cnt; s += kWarps) {
-      const float es = __shfl_sync(kAll, e, s);
-      const float* o = s0 + s < n_pre ? a.pre_out + (pre + s0 + s) * D
-                                      : a.tail_out + (own + s0 + s - n_pre) * D;
-      float v[kPer];
-      if constexpr (kPer == 2) {
-        const float2 u = reinterpret_cast<const float2*>(o)[lane];
-        v[0] = u.x;
-        v[1] = u.y;
-      } else {
+  const auto add = [&](float ls, const float* x) {
+    if (ls == -CUDART_INF_F) return;  // an empty part holds nothing (a NaN weight passes)
+    const float e = __expf(ls - m);
+    sum += e;
 #pragma unroll
-        for (int i = 0; i < kPer / 4; ++i) {
-          const float4 u = reinterpret_cast<const float4*>(o)[lane + 32 * i];
-          v[4 * i] = u.x;
-          v[4 * i + 1] = u.y;
-          v[4 * i + 2] = u.z;
-          v[4 * i + 3] = u.w;
-        }
-      }
-      sum += es;
-      if (es != 0.f)  // an empty part holds nothing (a NaN weight passes)
+    for (int i = 0; i < kPer; ++i) acc[i] = fmaf(e, x[i], acc[i]);
+  };
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) acc[i] = fmaf(es, v[i], acc[i]);
+  for (int i = 0; i < kAhead; ++i) {
+    const int s = w + i * kWarps;
+    if (s < 32) {
+      add(__shfl_sync(kAll, first, s), v[i]);
+    } else if (there(s)) {
+      add(lse_at(s), v[i]);
     }
+  }
+#pragma unroll 1
+  for (int s0 = w + kAhead * kWarps; s0 < total; s0 += kAhead * kWarps) {
+    float ls[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int s = s0 + i * kWarps;
+      ls[i] = -CUDART_INF_F;
+      if (there(s)) {
+        load(s, v[i]);
+        ls[i] = lse_at(s);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) add(ls[i], v[i]);
   }
   if constexpr (kWarps > 1) {
 #pragma unroll
@@ -827,13 +874,12 @@ __global__ void __launch_bounds__(kMergeThreads) merge_parts_kernel(const MergeA
     __syncthreads();
     if (w != 0) return;
 #pragma unroll
-    for (int o = 1; o < kWarps; ++o) {
-      sum += sum_s[warp + o];
+    for (int p = 1; p < kWarps; ++p) {
+      sum += sum_s[warp + p];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) acc[i] += acc_s[warp + o][i * 32 + lane];
+      for (int i = 0; i < kPer; ++i) acc[i] += acc_s[warp + p][i * 32 + lane];
     }
   }
-  if (!live) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* out = a.out + (size_t)row * D;
   if constexpr (kPer == 2) {
@@ -888,7 +934,7 @@ int launch_shared(const CUtensorMap* maps, const PrefixArgs& p, const MergeArgs&
   const char* name = "sc_shared_prefix_attention";
   using S = PrefixShape<D>;
   constexpr size_t tail_smem =
-      (size_t)kTailWarps * kTailStages * (2 * S::PAGE_BYTES + sizeof(uint64_t));
+      (size_t)kTailWarps * kTailStages * (2 * S::PAGE_BYTES + sizeof(uint64_t)) + 32 * sizeof(int);
   static int configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -919,11 +965,15 @@ int launch_shared(const CUtensorMap* maps, const PrefixArgs& p, const MergeArgs&
   err = launch_pdl(tail_kernel<D>, dim3(ctas, p.slabs), dim3(kTailWarps * 32), tail_smem, s, t);
   if (err != cudaSuccess)
     return set_error(SC_ERR_CUDA, "%s: launch: %s", name, cudaGetErrorString(err));
-  // A warp a row while the rows fill the GPU; few rows of many parts get eight.
-  const bool wide = m.rows * 8 <= 148 * 64 && m.pre_splits + m.tail_splits > 4;
-  const int per_cta = wide ? 1 : kMergeThreads / 32;
-  err = launch_pdl(wide ? merge_parts_kernel<D, 8> : merge_parts_kernel<D, 1>,
-                   dim3((m.rows + per_cta - 1) / per_cta), dim3(kMergeThreads), 0, s, m);
+  // As many warps a row (a power of two, at most 8) as the GPU holds at once.
+  const int fit = 148 * 40 / m.rows;
+  const int share = fit >= 8 ? 8 : fit >= 4 ? 4 : fit >= 2 ? 2 : 1;
+  const auto merge = share == 8   ? merge_parts_kernel<D, 8>
+                     : share == 4 ? merge_parts_kernel<D, 4>
+                     : share == 2 ? merge_parts_kernel<D, 2>
+                                  : merge_parts_kernel<D, 1>;
+  const int per_cta = kMergeThreads / 32 / share;
+  err = launch_pdl(merge, dim3((m.rows + per_cta - 1) / per_cta), dim3(kMergeThreads), 0, s, m);
   if (err != cudaSuccess)
     return set_error(SC_ERR_CUDA, "%s: launch: %s", name, cudaGetErrorString(err));
   return check_launch(name);

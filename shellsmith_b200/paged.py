@@ -429,7 +429,7 @@ class PrefixGroups:
             raise ValueError(f"PrefixGroups: head_dim must be 64, 128 or 256, got {head_dim}")
         self.batch, self.q_heads, self.kv_heads, self.head_dim = batch, q_heads, kv_heads, head_dim
         per_tile = PREFIX_ROWS // (q_heads // kv_heads)
-        first_page, tiles, members = [0] * batch, [], []
+        first_page, tiles, members, shared = [0] * batch, [], [], 0
         seen: set = set()
         for rows, tokens in groups:
             rows, pages = [int(r) for r in rows], int(tokens) // PAGE_SIZE
@@ -447,17 +447,33 @@ class PrefixGroups:
                 members += part
             for r in rows:
                 first_page[r] = pages
+            shared += pages
         self.ntiles = len(tiles)
         self.max_prefix_pages = max((t[2] for t in tiles), default=0)
-        self.min_first_page = min(first_page, default=0)
-        self.pages_per_split, self.num_splits = prefix_split_plan(
-            [t[2] for t in tiles], kv_heads, head_dim, sms or sm_count(device), pages_per_split)
+        self.shared_pages = shared
+        # Two splits of the prefix: where it is most of the work, and where the sequences'
+        # own pages are a good part of it (see splits()).
+        self.sms = sms = sms or sm_count(device)
+        self._splits = [prefix_split_plan([t[2] for t in tiles], kv_heads, head_dim, n,
+                                          pages_per_split) for n in (sms, max(1, sms * 7 // 9))]
         # One transfer: tiles [ntiles, 4], then first_page [batch], then members.
         flat = torch.tensor([x for t in tiles for x in t] + first_page + members,
                             dtype=torch.int32).to(device)
         self.tiles = flat[:4 * len(tiles)]
         self.first_page = flat[4 * len(tiles):4 * len(tiles) + batch]
         self.members = flat[4 * len(tiles) + batch:]
+        self.device_index = flat.get_device()
+        self.tiles_ptr, self.first_page_ptr, self.members_ptr = (
+            flat.data_ptr() + 4 * n for n in (0, 4 * len(tiles), 4 * len(tiles) + batch))
+
+    def splits(self, own_pages: int | None) -> tuple:
+        """(pages_per_split, num_splits) of the shared pages beside `own_pages` pages of the
+        sequences' own. From 30 % of the pages on, two ninths of the SMs are left to these
+        alone: 64 sequences of U[1, 2048] tokens on 8 prefixes of 16,272 took 74 us with 112
+        prefix CTAs and 77 with 144, 128 of U[1, 1024] on one of 8,208 49 and 53; 15 of
+        U[1, 777] on 3 of 5,104 (27 %) 25.4 with 96 and 24.5 with 120."""
+        busy = own_pages is None or 10 * own_pages >= 3 * (own_pages + self.shared_pages)
+        return self._splits[busy]
 
 
 def prefix_split_plan(tile_pages: list, kv_heads: int, head_dim: int, sms: int,
@@ -491,25 +507,29 @@ def tail_split_plan(batch: int, q_heads: int, kv_heads: int, max_pages: int,
 
 
 class SharedPrefixWorkspace:
-    """Reusable scratch of shared_prefix_attention (the partials); grows when needed."""
+    """Reusable scratch of shared_prefix_attention (the parts); grows when needed."""
 
     def __init__(self, device: str | torch.device = "cuda"):
         self.device = torch.device(device)
         self._buffer = torch.empty(0, dtype=torch.float32, device=device)
+        self._floats = 0
 
     def parts(self, rows: int, dim: int, prefix_splits: int, splits: int) -> tuple:
         """Addresses of prefix_out, prefix_lse, part_out, part_lse for `rows` (row, head)s,
         and of the work counters."""
-        sizes = [-(-n // 4) * 4 for n in (rows * prefix_splits * dim, rows * prefix_splits,
-                                          rows * splits * dim, rows * splits, rows // 1024 + 1)]
-        if self._buffer.numel() < sum(sizes):
-            self._buffer = torch.empty(sum(sizes), dtype=torch.float32, device=self.device)
-        at = self._buffer.data_ptr()
-        out = []
-        for n in sizes:
-            out.append(at)
-            at += 4 * n
-        return tuple(out)
+        pre, own = rows * prefix_splits, rows * splits
+        at1 = pre * dim                          # D is a multiple of 64: aligned steps
+        at2 = at1 + own * dim
+        need = at2 + pre + own + rows // 1024 + 1
+        if self._floats < need:
+            self._buffer = torch.empty(need, dtype=torch.float32, device=self.device)
+            self._floats = need
+        base = self._buffer.data_ptr()
+        return (base, base + 4 * at2, base + 4 * at1, base + 4 * (at2 + pre),
+                base + 4 * (at2 + pre + own))
+
+
+_shared_prefix = _capi.bind("sc_shared_prefix_attention")
 
 
 def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tensor,
@@ -548,10 +568,13 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
                                       max_pages_in_batch=max_suffix_pages,
                                       total_pages=total_suffix_pages, out=out, lse_out=lse_out,
                                       sms=sms)
+    if groups.device_index != q.get_device():
+        raise ValueError(f"the groups are on {groups.tiles.device}, q on {q.device}")
     pps, nsplit = tail_split_plan(B, hq, hkv, max_suffix_pages or max_pages, pages_per_split,
-                                  total_suffix_pages, sms or sm_count(q.device))
+                                  total_suffix_pages, sms or groups.sms)
+    pre_pps, pre_splits = groups.splits(total_suffix_pages)
     if out is None:
-        out = torch.empty((B, hq, dim), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((B, hq, dim))
     else:
         require_cuda("out", out, torch.bfloat16, 3)
         if out.shape != q.shape:
@@ -562,13 +585,13 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
             raise ValueError("shared_prefix_attention: lse_out must be [B * Hq]")
     if workspace is None:
         workspace = SharedPrefixWorkspace(q.device)
-    pre_out, pre_lse, part_out, part_lse, counters = workspace.parts(B * hq, dim, groups.num_splits, nsplit)
-    _capi.call("sc_shared_prefix_attention", ptr(q), ptr(kv_pool), num_pages, ptr(block_table),
-               ptr(ctx_len), ptr(groups.first_page), ptr(groups.tiles),
-               ptr(groups.members), groups.ntiles, B, hq, hkv, dim, page, max_pages,
-               groups.pages_per_split, groups.num_splits, pps, nsplit, float(scale), pre_out,
-               pre_lse, part_out, part_lse, counters, ptr(out), ptr(lse_out), stream_of(q))
-    _count(3 if B else 0)
+    _shared_prefix(q.data_ptr(), kv_pool.data_ptr(), num_pages, block_table.data_ptr(),
+                   ctx_len.data_ptr(), groups.first_page_ptr, groups.tiles_ptr,
+                   groups.members_ptr, groups.ntiles, B, hq, hkv, dim, page, max_pages, pre_pps,
+                   pre_splits, pps, nsplit, scale,
+                   *workspace.parts(B * hq, dim, pre_splits, nsplit), out.data_ptr(),
+                   ptr(lse_out), stream_of(q))
+    _count(3)
     return out
 
 

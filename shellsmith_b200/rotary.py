@@ -14,6 +14,7 @@ packed prompts alike:
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -69,7 +70,11 @@ def axis_of_pairs(sections, interleaved: bool) -> list:
 
 
 _append = _capi.bind("sc_rotary_append")
-_Strides = ctypes.c_int64 * 6
+
+
+@functools.lru_cache(maxsize=256)
+def _strides(*values) -> ctypes.Array:
+    return (ctypes.c_int64 * 6)(*values)
 
 
 def _operand(name: str, t: torch.Tensor, dim: int) -> tuple:
@@ -112,7 +117,7 @@ def _run(q, k, v, k_shape, strides, positions, plan, q_weight, k_weight, eps, q_
                          f"got {positions.dtype} {tuple(positions.shape)}")
     if plan.device_index != q.get_device():
         raise ValueError(f"the plan is on {plan.turns.device}, q on {q.device}")
-    _append(q.data_ptr(), k.data_ptr(), v, _Strides(*strides), positions.data_ptr(), pos_stride[0],
+    _append(q.data_ptr(), k.data_ptr(), v, _strides(*strides), positions.data_ptr(), pos_stride[0],
             plan.axes, plan.turns_ptr, plan.axis_ptr, _weight("q_weight", q_weight, dim),
             _weight("k_weight", k_weight, dim), eps, q_out.data_ptr(), k_out, pool, slots, ntok,
             q.shape[1], k_shape[1], dim, plan.rotary_dim, page, pages, stream_of(q))
