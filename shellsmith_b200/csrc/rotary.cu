@@ -15,12 +15,13 @@
 // double, so the reduction is one multiply and one subtraction of the nearest whole
 // turn; sine and cosine of the remaining fraction are fp32.
 //
-// B200 mapping. HBM-bound: each value is read and written once. A CTA makes the
-// (cos, sin) table of its tokens in shared memory, then its warps walk the tokens'
-// head rows (q, k, v). D / 8 lanes hold a row, 8 values each as two 4-value pieces: a
-// lane of the rotary part holds both halves of four pairs, so that a turn needs no
-// exchange, and the norm is a shuffle sum. Two rows are loaded before the first is
-// computed; the norm's weights stay in registers.
+// B200 mapping. HBM-bound: each value is read and written once. A CTA makes the (cos, sin)
+// table of its tokens in shared memory, then each of its warps takes heads and walks the
+// tokens of one, four rows loaded before the first is computed. D / 8 lanes hold a row, 8
+// values each as two 4-value pieces: a lane of the rotary part holds both halves of four
+// pairs, so that a turn needs no exchange, and the norm is a shuffle sum. Products go two
+// at a time (fp32 pairs).
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -29,7 +30,7 @@ namespace sc {
 namespace {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotTokens = 4;      // tokens of one CTA on long inputs
+constexpr int kRotTokens = 32;     // most tokens of one CTA
 
 struct RotaryArgs {
   const uint16_t *q, *k, *v;
@@ -64,14 +65,36 @@ __device__ __forceinline__ void unpack4(const uint2& u, float* x) {
   x[3] = bf16_hi(u.y);
 }
 
+// Two fp32 values in one register pair: one instruction for two products.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
 template <int D, bool kVec>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a, int tokens) {
+__global__ void __launch_bounds__(kRotThreads, 4)
+    rotary_kernel(const __grid_constant__ RotaryArgs a, int tokens) {
   constexpr int kLanes = D / 8;              // lanes of one row
   constexpr int kRows = 32 / kLanes;         // rows of one warp
   constexpr int kStep = kRotThreads / 32 * kRows;
-  constexpr int kAhead = 2;                  // rows in flight per lane
-  extern __shared__ float4 table4[];         // [tokens][half] (cos, sin)
-  float2* table = reinterpret_cast<float2*>(table4);
+  constexpr int kAhead = 4;                  // rows in flight per lane
+  extern __shared__ float4 table[];          // [tokens][half / 4] x (4 cos, 4 sin)
+  __shared__ long long pool_row[kRotTokens]; // where a token's rows start in the pool, or -1
+  __shared__ int pool_flip[kRotTokens];      // and how its 16-byte chunks are permuted
   pdl_wait();
   pdl_trigger();
   const int t0 = blockIdx.x * tokens;
@@ -82,7 +105,18 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a,
     const double turn = (double)a.positions[ax * a.pos_axis + t0 + t] * a.turns[p];
     float s, c;
     sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
-    table[i] = make_float2(c, s);
+    float* at = reinterpret_cast<float*>(table) + 2 * (i - (p & 3)) + (p & 3);
+    at[0] = c;
+    at[4] = s;
+  }
+  if (a.pool != nullptr && threadIdx.x < nt) {
+    const int64_t slot = a.slots[t0 + threadIdx.x];
+    const int64_t page = slot >> a.page_shift;
+    const int off = (int)slot & (a.P - 1);
+    const bool in = slot >= 0 && page < a.num_pages;
+    if (slot >= 0 && !in) flag_device(a.status, DEV_BAD_INDEX);
+    pool_row[threadIdx.x] = in ? (page * a.Hkv * 2 * a.P + off) * D : -1;
+    pool_flip[threadIdx.x] = 8 * (off & 7);
   }
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -91,126 +125,130 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a,
   // neighbours. lo / hi are their first elements.
   const int turning = a.half / 4;            // lanes of the rotary part
   const bool turns = c < turning;
-  const int lo = turns ? 4 * c : 8 * c;  // 2 half + 8 (c - half / 4)
+  const int lo = turns ? 4 * c : 8 * c;      // 2 half + 8 (c - half / 4)
   const int hi = turns ? lo + a.half : lo + 4;
-
-  // The rows (token, head) of one operand, kStep * gridDim.y apart for this lane's; kKind:
-  // 0 q, 1 k, 2 v. All lanes of a warp go around alike: the shuffles want the whole warp.
+  // Heads of one operand, a head (kRows of them) to a warp, its tokens one after the
+  // other; kKind: 0 q, 1 k, 2 v. All lanes of a warp go around alike: the shuffles want
+  // the whole warp. Operands start on different warps (skew).
   const auto walk = [&](auto kind, int nheads, int skew, const uint16_t* in, long long in_tok,
-                        long long in_head, const float* w, bool norm) {
+                        long long in_head, const uint16_t* weight) {
     constexpr int kKind = decltype(kind)::value;
     const int step = kStep * gridDim.y;
-    // Operands start on different warps, so that a few heads do not all fall on the first.
     int h = ((blockIdx.y * (kRotThreads / 32) + warp) * kRows + lane / kLanes + step - skew) % step;
-    int t = 0;
-    const auto settle = [&]() {
-      while (h >= nheads) {
-        h -= nheads;
-        ++t;
-      }
-    };
-    settle();
-    while (__any_sync(0xffffffffu, t < nt)) {
-      uint2 u[kAhead][2];
-      uint16_t* dst[kAhead];
-      int tt[kAhead], flip[kAhead];
+    if (!__any_sync(0xffffffffu, h < nheads)) return;
+    uint64_t w[4];
+    if (weight != nullptr) {
+      float f[8];
+      unpack4(*reinterpret_cast<const uint2*>(weight + lo), f);
+      unpack4(*reinterpret_cast<const uint2*>(weight + hi), f + 4);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        tt[i] = t;
-        flip[i] = 0;
-        dst[i] = nullptr;
-        u[i][0] = u[i][1] = make_uint2(0u, 0u);
-        if (t < nt) {
-          const int tok = t0 + t;
-          if constexpr (kKind == 0) {
-            dst[i] = a.q_out + ((size_t)tok * nheads + h) * D;
-          } else if (a.pool != nullptr) {
-            const int64_t slot = a.slots[tok];
-            const int64_t page = slot >> a.page_shift;
-            if (slot >= 0 && page < a.num_pages) {
-              const int off = (int)slot & (a.P - 1);
-              dst[i] = a.pool + ((((size_t)page * nheads + h) * 2 + (kKind == 2)) * a.P + off) * D;
-              flip[i] = 8 * (off & 7);  // 16-byte chunks move, halves of one stay
-            } else if (slot >= 0 && c == 0) {
-              flag_device(a.status, DEV_BAD_INDEX);
-            }
-          } else if constexpr (kKind == 1) {
-            dst[i] = a.k_out + ((size_t)tok * nheads + h) * D;
-          }
-          if (dst[i] != nullptr) {
-            const uint16_t* src = in + tok * in_tok + h * in_head;
+      for (int e = 0; e < 4; ++e) w[e] = pair(f[2 * e], f[2 * e + 1]);
+    }
+    for (; __any_sync(0xffffffffu, h < nheads); h += step) {
+      const bool live = h < nheads;
+      const uint16_t* src = in + t0 * in_tok + (live ? h : 0) * in_head;
+      uint16_t* out = kKind == 0 ? a.q_out + ((size_t)t0 * nheads + h) * D
+                                 : (kKind == 1 && a.pool == nullptr
+                                        ? a.k_out + ((size_t)t0 * nheads + h) * D
+                                        : a.pool + (size_t)(2 * h + (kKind == 2)) * a.P * D);
+      for (int tb = 0; tb < nt; tb += kAhead) {
+        uint2 u[kAhead][2];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          u[i][0] = u[i][1] = make_uint2(0u, 0u);
+          if (live && tb + i < nt) {
             u[i][0] = load4<kVec>(src + lo);
             u[i][1] = load4<kVec>(src + hi);
           }
+          src += in_tok;
         }
-        h += step;
-        settle();
-      }
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if constexpr (kKind != 2) {
-          float x[8];
-          unpack4(u[i][0], x);
-          unpack4(u[i][1], x + 4);
-          if (norm) {
-            float sum = 0.f;
+        for (int i = 0; i < kAhead; ++i) {
+          const int t = tb + i;
+          if (t >= nt) break;  // uniform
+          if constexpr (kKind != 2) {
+            float f[8];
+            unpack4(u[i][0], f);
+            unpack4(u[i][1], f + 4);
+            uint64_t x[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+            for (int e = 0; e < 4; ++e) x[e] = pair(f[2 * e], f[2 * e + 1]);
+            if (weight != nullptr) {
+              uint64_t sq = mul2(x[0], x[0]);
 #pragma unroll
-            for (int off = kLanes / 2; off >= 1; off >>= 1)
-              sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            const float inv = rsqrtf(sum * (1.f / D) + a.eps);
+              for (int e = 1; e < 4; ++e) sq = fma2(x[e], x[e], sq);
+              float s0, s1;
+              unpair(sq, s0, s1);
+              float sum = s0 + s1;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
-          }
-          if (turns && tt[i] < nt) {
-            const float4* cs = table4 + (tt[i] * a.half + 4 * c) / 2;
-            const float4 p = cs[0], r = cs[1];
-            const float co[4] = {p.x, p.z, r.x, r.z}, si[4] = {p.y, p.w, r.y, r.w};
+              for (int off = kLanes / 2; off >= 1; off >>= 1)
+                sum += __shfl_xor_sync(0xffffffffu, sum, off);
+              const float inv = rsqrtf(sum * (1.f / D) + a.eps);
+              const uint64_t both = pair(inv, inv);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y = x[e], z = x[4 + e];
-              x[e] = y * co[e] - z * si[e];
-              x[4 + e] = z * co[e] + y * si[e];
+              for (int e = 0; e < 4; ++e) x[e] = mul2(mul2(x[e], both), w[e]);
             }
+            if (turns) {
+              const float4 co = table[2 * (t * turning + c)], si = table[2 * (t * turning + c) + 1];
+              const uint64_t c0 = pair(co.x, co.y), c1 = pair(co.z, co.w);
+              const uint64_t s0 = pair(si.x, si.y), s1 = pair(si.z, si.w);
+              const uint64_t n0 = pair(-si.x, -si.y), n1 = pair(-si.z, -si.w);
+              const uint64_t y0 = x[0], y1 = x[1], z0 = x[2], z1 = x[3];
+              x[0] = fma2(y0, c0, mul2(z0, n0));
+              x[1] = fma2(y1, c1, mul2(z1, n1));
+              x[2] = fma2(z0, c0, mul2(y0, s0));
+              x[3] = fma2(z1, c1, mul2(y1, s1));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) unpair(x[e], f[2 * e], f[2 * e + 1]);
+            u[i][0] = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+            u[i][1] = make_uint2(pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
           }
-          u[i][0] = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-          u[i][1] = make_uint2(pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-        }
-        if (dst[i] != nullptr) {
-          *reinterpret_cast<uint2*>(dst[i] + (lo ^ flip[i])) = u[i][0];
-          *reinterpret_cast<uint2*>(dst[i] + (hi ^ flip[i])) = u[i][1];
+          if constexpr (kKind == 0) {
+            if (live) {
+              *reinterpret_cast<uint2*>(out + lo) = u[i][0];
+              *reinterpret_cast<uint2*>(out + hi) = u[i][1];
+            }
+            out += (size_t)nheads * D;
+          } else if (a.pool != nullptr) {
+            const long long row = pool_row[t];
+            if (live && row >= 0) {  // 16-byte chunks move, halves of one stay
+              const int flip = pool_flip[t];
+              *reinterpret_cast<uint2*>(out + row + (lo ^ flip)) = u[i][0];
+              *reinterpret_cast<uint2*>(out + row + (hi ^ flip)) = u[i][1];
+            }
+          } else {
+            if (live) {
+              *reinterpret_cast<uint2*>(out + lo) = u[i][0];
+              *reinterpret_cast<uint2*>(out + hi) = u[i][1];
+            }
+            out += (size_t)nheads * D;
+          }
         }
       }
     }
   };
-  float w[8];
-  const auto weights = [&](const uint16_t* p) {
-    if (p == nullptr) return;
-    unpack4(*reinterpret_cast<const uint2*>(p + lo), w);
-    unpack4(*reinterpret_cast<const uint2*>(p + hi), w + 4);
-  };
-  weights(a.q_weight);
   __syncthreads();
-  walk(std::integral_constant<int, 0>{}, a.Hq, 0, a.q, a.q_tok, a.q_head, w, a.q_weight != nullptr);
-  weights(a.k_weight);
   const int step = kStep * gridDim.y;
-  walk(std::integral_constant<int, 1>{}, a.Hkv, nt * a.Hq % step, a.k, a.k_tok, a.k_head, w,
-       a.k_weight != nullptr);
+  walk(std::integral_constant<int, 0>{}, a.Hq, 0, a.q, a.q_tok, a.q_head, a.q_weight);
+  walk(std::integral_constant<int, 1>{}, a.Hkv, a.Hq % step, a.k, a.k_tok, a.k_head, a.k_weight);
   if (a.pool != nullptr)
-    walk(std::integral_constant<int, 2>{}, a.Hkv, nt * (a.Hq + a.Hkv) % step, a.v, a.v_tok, a.v_head,
-         w, false);
+    walk(std::integral_constant<int, 2>{}, a.Hkv, (a.Hq + a.Hkv) % step, a.v, a.v_tok, a.v_head,
+         static_cast<const uint16_t*>(nullptr));
 }
 
 template <int D>
 cudaError_t launch_rotary(const RotaryArgs& a, bool vec, cudaStream_t s) {
-  // Few tokens: one token a CTA and its heads spread over CTAs, so that every warp has
-  // about one row; many: kRotTokens tokens a CTA.
+  // Tokens of a CTA: as few as fill the GPU (four CTAs an SM), in whole waves of CTAs; few
+  // tokens spread their heads over CTAs, so that a warp has about one row.
+  constexpr long long kFit = 148 * 4;
   const int rows_per_cta = kRotThreads / 32 * (32 / (D / 8));
   const int heads = a.Hq + 2 * a.Hkv;
-  const bool few = a.ntok <= 1024;
-  const int tokens = few ? 1 : kRotTokens;
-  const dim3 grid((a.ntok + tokens - 1) / tokens, few ? (heads + rows_per_cta - 1) / rows_per_cta : 1);
+  const long long waves = (a.ntok + kFit * kRotTokens - 1) / (kFit * kRotTokens);
+  const int tokens = (int)((a.ntok + kFit * waves - 1) / (kFit * waves));
+  const int ctas = (a.ntok + tokens - 1) / tokens;
+  const int spread = (heads + rows_per_cta - 1) / rows_per_cta;
+  const dim3 grid(ctas, (int)std::max(1ll, std::min<long long>(spread, kFit / ctas)));
   const size_t smem = (size_t)tokens * a.half * sizeof(float2);
   return launch_pdl(vec ? rotary_kernel<D, true> : rotary_kernel<D, false>, grid,
                     dim3(kRotThreads), smem, s, a, tokens);
