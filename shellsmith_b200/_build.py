@@ -1,15 +1,18 @@
-"""Builds libshellcache.so (the C ABI) in-tree with nvcc for sm_100a only."""
+"""Builds libshellcache.so (the C ABI) in-tree with nvcc for sm_100a only, and beside it
+_fastpath.so, the callers of the group-decode operators (needs torch and Python headers)."""
 
 from __future__ import annotations
 
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 LIBRARY = PACKAGE / "libshellcache.so"
+FASTPATH = PACKAGE / "_fastpath.so"
 SOURCES = ("status.cu", "gdn_decode.cu", "gdn_front.cu", "gdn_chunk.cu", "paged_kv.cu",
            "paged_attention.cu", "paged_q8.cu", "exchange.cu", "shared_prefix.cu", "rotary.cu",
            "beam.cu")
@@ -32,9 +35,35 @@ def _stale() -> bool:
     return any(p.stat().st_mtime > built for p in inputs if p.exists())
 
 
+def _build_fastpath(force: bool, verbose: bool) -> None:
+    """Compile the callers (csrc/fastpath.cpp) against torch; they link the library."""
+    inputs = [CSRC / "fastpath.cpp", PACKAGE.parent / "include" / "shellcache.h"]
+    if not force and FASTPATH.exists() and all(p.stat().st_mtime <= FASTPATH.stat().st_mtime
+                                               for p in inputs):
+        return
+    import torch
+
+    base = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = FASTPATH.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{base}/include", f"-I{base}/include/torch/csrc/api/include",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", str(inputs[0]),
+           "-o", str(tmp), f"-L{PACKAGE}", "-l:libshellcache.so", f"-L{base}/lib", "-lc10",
+           "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd))
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stderr[-4000:]}")
+    os.replace(tmp, FASTPATH)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile every kernel source into one shared library next to this file."""
     if not force and not _stale():
+        _build_fastpath(False, verbose)
         return LIBRARY
     tmp = LIBRARY.with_suffix(".so.tmp")
     cmd = [
@@ -48,6 +77,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if proc.returncode != 0:
         raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stderr[-4000:]}")
     os.replace(tmp, LIBRARY)
+    _build_fastpath(force, verbose)
     return LIBRARY
 
 

@@ -20,6 +20,14 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+# The compiled callers of the group-decode operators (csrc/fastpath.cpp), or None where
+# they are not built: the wrappers then make the same calls themselves.
+try:
+    from . import _fastpath as fast
+except ImportError:
+    fast = None
+
+
 def require_cuda(name: str, t: torch.Tensor, dtype: torch.dtype, ndim: int | None = None,
                  align: int = 16) -> None:
     """Check device, dtype, rank, contiguity and alignment of a kernel operand."""

@@ -20,7 +20,7 @@ import numpy as np
 import torch
 
 from . import _capi
-from ._torch import ptr, require_cuda, stream_of
+from ._torch import fast, ptr, require_cuda, stream_of
 
 MAX_BEAMS = 64   # beams of one group
 MAX_SELECT = 64  # continuations asked for at once
@@ -48,6 +48,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, *,
     continuations have a score above -inf, those of lowest index follow with -inf (a NaN
     score counts as -inf).
     """
+    if fast is not None:
+        done = fast.beam_select(logits, scores, n, finished, pad_token)
+        if done is not None:
+            return done
     if not isinstance(logits, torch.Tensor) or logits.dim() != 3:
         raise ValueError("beam_select: logits must be a [groups, beams, vocab] tensor")
     if not logits.is_cuda:
@@ -92,11 +96,16 @@ def reorder_rows(pools, slots: torch.Tensor, parents: torch.Tensor) -> torch.Ten
     keeps the beam's row, each later child gets a copy in the row of a beam without
     children (ascending), so nothing else moves. slots, parents, result: int32 [G, K].
     """
+    if fast is not None:
+        done = fast.reorder_rows(pools, slots, parents)
+        if done is not None:
+            return done
     require_cuda("slots", slots, torch.int32, 2, align=4)
     require_cuda("parents", parents, torch.int32, 2, align=4)
     groups, beams = shape = slots.shape
     if parents.shape != shape:
         raise ValueError("reorder_rows: slots and parents must have the same shape")
+    pools = list(pools)
     count = len(pools)
     if count > 4:
         raise ValueError(f"reorder_rows: at most 4 pools, got {count}")

@@ -28,7 +28,7 @@ import math
 import torch
 
 from . import _capi
-from ._torch import ptr, require_cuda, stream_of
+from ._torch import fast, ptr, require_cuda, stream_of
 
 PAGE_SIZE = 16
 
@@ -465,6 +465,9 @@ class PrefixGroups:
         self.device_index = flat.get_device()
         self.tiles_ptr, self.first_page_ptr, self.members_ptr = (
             flat.data_ptr() + 4 * n for n in (0, 4 * len(tiles), 4 * len(tiles) + batch))
+        self.packed = (batch, q_heads, kv_heads, head_dim, self.device_index, self.ntiles,
+                       self.max_prefix_pages, self.first_page_ptr, self.tiles_ptr,
+                       self.members_ptr)
 
     def splits(self, own_pages: int | None) -> tuple:
         """(pages_per_split, num_splits) of the shared pages beside `own_pages` pages of the
@@ -549,6 +552,17 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
     group); when omitted the block-table width bounds them. lse_out [B * Hq] fp32. bf16
     pools only. Calls that share a workspace must not overlap on the GPU.
     """
+    if fast is not None and workspace is not None and groups.ntiles:
+        pre = groups.splits(total_suffix_pages)
+        tail = tail_split_plan(groups.batch, groups.q_heads, groups.kv_heads,
+                               max_suffix_pages or block_table.shape[1], pages_per_split,
+                               total_suffix_pages, sms or groups.sms)
+        done = fast.shared_prefix_attention(
+            q, kv_pool, block_table, ctx_len, scale, out, lse_out, groups.packed, pre, tail,
+            workspace.parts(groups.batch * groups.q_heads, groups.head_dim, pre[1], tail[1]))
+        if done is not None:
+            _count(3)
+            return done
     if kv_pool.dtype != torch.bfloat16:
         raise TypeError("shared_prefix_attention takes bf16 pools")
     num_pages, hkv, page, dim = _pool_dims(kv_pool)

@@ -20,7 +20,7 @@ import math
 import torch
 
 from . import _capi, paged
-from ._torch import require_cuda, stream_of
+from ._torch import fast, require_cuda, stream_of
 
 
 class RotaryPlan:
@@ -59,6 +59,7 @@ class RotaryPlan:
         self.turns = (self.inv_freq / (2 * math.pi)).to(device)  # whole turns per position
         self.device_index = self.turns.get_device()
         self.turns_ptr, self.axis_ptr = self.turns.data_ptr(), self.axis.data_ptr()
+        self.packed = (head_dim, rot, self.axes, self.turns_ptr, self.axis_ptr, self.device_index)
 
 
 def axis_of_pairs(sections, interleaved: bool) -> list:
@@ -149,6 +150,11 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     its q is still turned). An 8-bit pool takes the turned k from a scratch tensor
     through its own append kernel (two launches).
     """
+    if fast is not None:
+        done = fast.rotary_append(q, k, v, positions, kv_pool, slot_mapping, q_weight, k_weight,
+                                  eps, out, plan.packed)
+        if done is not None:
+            return done
     q_shape, qs = _operand("q", q, plan.head_dim)
     k_shape, ks = _operand("k", k, plan.head_dim)
     v_shape, vs = _operand("v", v, plan.head_dim)
