@@ -58,6 +58,7 @@ class BlockManager:
         self.pages: dict[int, list] = {}
         self.owner: dict[int, object] = {}
         self.dirty_rows: set = set()
+        self.sharing = 0  # counts the changes of which sequences share which pages
 
     # ------------------------------------------------------------ queries
     @property
@@ -98,6 +99,7 @@ class BlockManager:
             raise OutOfPages(f"{need} pages needed, {len(self._free_pages)} free")
         slot = heapq.heappop(self._free_slots)
         pages = self.take_pages(need)
+        self.sharing += 1
         self.pages[slot] = pages
         self.owner[slot] = owner
         self.table[slot, :need] = pages
@@ -175,6 +177,7 @@ class BlockManager:
         if len(pages) > self.max_pages_per_seq or self.pages_for(tokens) != len(pages):
             raise ValueError("adopt: page count does not match the token count")
         slot = heapq.heappop(self._free_slots)
+        self.sharing += 1
         self.pages[slot] = list(pages)
         self.owner[slot] = owner
         self.table[slot, :len(pages)] = pages
@@ -183,6 +186,35 @@ class BlockManager:
         self.active[slot] = True
         self.dirty_rows.add(slot)
         return slot
+
+    def replace(self, slot: int, pages: list, tokens: int) -> None:
+        """Give an active slot other pages, which the caller owns already (a beam that
+        continues another one); its old pages lose an owner."""
+        if len(pages) > self.max_pages_per_seq or self.pages_for(tokens) != len(pages):
+            raise ValueError("replace: page count does not match the token count")
+        old, self.pages[slot] = self.pages[slot], list(pages)
+        self.drop(old)
+        self.sharing += 1
+        self.table[slot, :len(pages)] = pages
+        self.table[slot, len(pages):] = 0
+        self.lengths[slot] = tokens
+        self.dirty_rows.add(slot)
+
+    def common_prefixes(self) -> list:
+        """[(slots, pages)]: active sequences that start with the same pages, two at least,
+        with the number of leading pages that all of them share."""
+        by_first: dict = {}
+        for slot in np.flatnonzero(self.active).tolist():
+            if self.pages[slot]:
+                by_first.setdefault(self.pages[slot][0], []).append(slot)
+        groups = []
+        for slots in by_first.values():
+            if len(slots) < 2:
+                continue
+            n = min(len(self.pages[s]) for s in slots)
+            same = (self.table[slots, :n] == self.table[slots[0], :n]).all(0)
+            groups.append((slots, int(n if same.all() else np.argmin(same))))
+        return groups
 
     def extend(self, slot: int, tokens: int) -> None:
         """Grow a sequence to `tokens` cached tokens (the rest of a prompt after a
@@ -203,6 +235,7 @@ class BlockManager:
     def release(self, slot: int) -> None:
         """Drop a sequence's pages (freed when no snapshot shares them) and free its slot."""
         pages = self.pages.pop(slot)
+        self.sharing += 1
         self.drop(pages)
         self.owner.pop(slot, None)
         self.lengths[slot] = 0

@@ -16,6 +16,11 @@ the caches are persistent device pools and one launch covers every row:
 A sequence's slot is its batch row, its block-table row and its GDN state row,
 so no gather/scatter of caches happens per step; inactive rows are skipped by
 the kernels (state slot -1, slot mapping -1, context length 0).
+
+Several sequences over one prompt (samples, beams): fork() shares its pages,
+append_rotary() and group_attention_layer() run an attention layer's step with the
+shared pages read once for all of them, and reorder() lets the sequences follow their
+beams (GDN state, taps and pages).
 Projections, norms and the MLP are outside the cache path and are not run.
 """
 
@@ -27,7 +32,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from . import gdn_layer, numerics, paged
+from . import beam, gdn_layer, numerics, paged, rotary
 from .block_manager import BlockManager
 
 
@@ -154,6 +159,9 @@ class HybridCacheEngine:
                                                   device=dev)
         self.max_pages_in_batch = 1
         self.total_pages = 0
+        self._group_ws = paged.SharedPrefixWorkspace(dev)
+        self._groups = None           # PrefixGroups of the batch, for ...
+        self._groups_for = None       # ... this state of the block manager
         self.rows = cfg.max_seqs  # rows the step's kernels cover (set by begin_step)
 
     # ------------------------------------------------------------ lifecycle
@@ -241,6 +249,44 @@ class HybridCacheEngine:
         self.blocks.drop(snap.pages)
         self._free_snapshot_rows.append(snap.row)
         snap.row = None
+
+    def reorder(self, slots, parents) -> list:
+        """Let the sequences in `slots` follow their beams: the j-th continues what
+        slots[parents[j]] holds. Returns the new slots.
+
+        The first child of a beam keeps its slot; each later one takes the slot of a beam
+        without children (beam.reorder_rows' rule): its GDN state and tap rows are copied
+        there on the device, full pages are shared and the partial last page is copied.
+        """
+        slots, parents = [int(s) for s in slots], [int(p) for p in parents]
+        if len(parents) != len(slots) or any(p < 0 or p >= len(slots) for p in parents):
+            raise ValueError("reorder: one parent among the slots for each of them")
+        if len(set(slots)) != len(slots) or not all(self.blocks.active[s] for s in slots):
+            raise ValueError("reorder: the slots must be distinct and hold sequences")
+        new, copies = beam.plan_reorder(slots, parents)
+        if not copies:
+            return new.tolist()
+        P, blocks = self.cfg.page_size, self.blocks
+        partial = sum(int(blocks.lengths[s]) % P != 0 for s, _ in copies)
+        if partial > blocks.free_pages:  # before anything changes
+            raise MemoryError(f"{partial} pages needed, {blocks.free_pages} free")
+        tables = torch.tensor([slots, parents], dtype=torch.int32, device=self.device)
+        pools = [self.state] if self.taps is None else [self.state, self.taps]
+        beam.reorder_rows(pools, tables[:1], tables[1:])
+        src, dst = [], []
+        for source, to in copies:
+            tokens = int(blocks.lengths[source])
+            pages = blocks.pages[source][:blocks.pages_for(tokens)]
+            owned = pages[:tokens // P]
+            blocks.share(owned)
+            if tokens % P:
+                fresh = blocks.take_pages(1)
+                src.append(pages[tokens // P])
+                dst += fresh
+                owned = owned + fresh
+            blocks.replace(to, owned, tokens)
+        self._copy_pages(src, dst)
+        return new.tolist()
 
     def cache_bytes(self, tokens: int) -> int:
         """Bytes a cache of `tokens` tokens holds: K/V of every attention layer plus the
@@ -400,6 +446,51 @@ class HybridCacheEngine:
                                 pages_per_split=self.cfg.pages_per_split,
                                 total_pages=self.total_pages, workspace=self.workspace,
                                 out=out[:n], seq_order=self.seq_order[:n], sms=self.cfg.sms)
+
+    def append_rotary(self, layer: int, q, k, v, plan: rotary.RotaryPlan, positions=None,
+                      q_weight=None, k_weight=None, eps: float = 1e-6) -> torch.Tensor:
+        """Norm and turn the staged rows' q and k and append k, v to their pages
+        (rotary.rotary_append); returns q. positions [axes, rows] int32 (default: each
+        row's own position on every axis)."""
+        n = self.rows
+        if positions is None:
+            positions = self.position[None, :n].expand(plan.axes, n)
+        return rotary.rotary_append(q[:n], k[:n], v[:n], positions, plan,
+                                    self.kv[self.attn_index[layer]], self.slot_map[:n],
+                                    q_weight=q_weight, k_weight=k_weight, eps=eps)
+
+    def prefix_groups(self) -> paged.PrefixGroups:
+        """The staged batch's sequences that share leading pages, laid out for
+        group_attention_layer; made anew when sequences come, go or change places."""
+        now = (self.rows, self.blocks.sharing)
+        if self._groups_for != now:
+            shared = [(slots, pages * self.cfg.page_size)
+                      for slots, pages in self.blocks.common_prefixes()]
+            self._groups = paged.PrefixGroups(shared, self.rows, self.cfg.q_heads,
+                                              self.cfg.kv_heads, self.cfg.head_dim,
+                                              device=self.device, sms=self.cfg.sms)
+            self._groups_for = now
+            first = np.zeros(self.rows, np.int64)
+            for slots, pages in shared:
+                first[slots] = pages
+            self._first_page = first
+        return self._groups
+
+    def group_attention_layer(self, layer: int, q, out) -> None:
+        """Attend over each staged row's pages, already holding its new token, the pages
+        that sequences share read once for all of them (paged.shared_prefix_attention)."""
+        n = self.rows
+        if n == 0:
+            return
+        groups = self.prefix_groups()
+        lengths = self._n_ctx[:n].astype(np.int64)
+        skip = np.minimum(self._first_page, lengths // self.cfg.page_size)
+        own = -(-lengths // self.cfg.page_size) - skip
+        paged.shared_prefix_attention(q[:n], self.kv[self.attn_index[layer]], self.table[:n],
+                                      self.ctx_len[:n], self.scale, groups,
+                                      max_suffix_pages=max(1, int(own.max())),
+                                      total_suffix_pages=int(own.sum()),
+                                      workspace=self._group_ws, out=out[:n], sms=self.cfg.sms)
 
     def decode_step(self, inputs: dict, outputs: dict) -> None:
         """Run every layer's cache work for the staged token of each active row.
