@@ -14,17 +14,22 @@ returns an alias of its inputs, so the ones the reference names with a
   shellcache::kv_append                  sc_kv_append / _q8
   shellcache::paged_decode_attention     sc_paged_decode_attention / _q8
   shellcache::paged_decode_attention_fused  append + split-K + merge in one launch
+  shellcache::rotary_append              sc_rotary (rotary.rotary_append)
+  shellcache::shared_prefix_attention    sc_shared_prefix_attention
+  shellcache::beam_select                sc_beam_select
+  shellcache::reorder_rows               sc_reorder_rows
 
 Importing this module registers the operators (once per process).
 """
 
 from __future__ import annotations
 
-from typing import Optional
+import functools
+from typing import List, Optional, Tuple
 
 import torch
 
-from . import numerics, paged
+from . import beam, numerics, paged, rotary
 
 _LIB = "shellcache"
 
@@ -144,3 +149,91 @@ def _(q, k_new, v_new, slot_mapping, kv_pool, block_table, ctx_len, scale,
 
 OPERATORS = ("gdn_decode", "gated_delta_token", "gated_delta_chunked", "gated_delta_chunks",
              "kv_append", "paged_decode_attention", "paged_decode_attention_fused")
+
+
+# ---- group decode: several continuations of shared prompts in one step
+@torch.library.custom_op(f"{_LIB}::rotary_append", mutates_args=("kv_pool",))
+def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                  kv_pool: torch.Tensor, slot_mapping: torch.Tensor, rotary_dim: int,
+                  base: float = 10000.0, sections: Optional[List[int]] = None,
+                  interleaved: bool = False, q_weight: Optional[torch.Tensor] = None,
+                  k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """Norm and turn q, k by positions [axes, ntok] and append k, v; returns q."""
+    plan = _plan(q.shape[-1], rotary_dim, base, tuple(sections) if sections else None,
+                 interleaved, q.device)
+    return rotary.rotary_append(q, k, v, positions, plan, kv_pool, slot_mapping,
+                                q_weight=q_weight, k_weight=k_weight, eps=eps)
+
+
+@functools.lru_cache(maxsize=32)
+def _plan(head_dim, rotary_dim, base, sections, interleaved, device) -> rotary.RotaryPlan:
+    """A plan is a function of these values alone: made once for each."""
+    return rotary.RotaryPlan(head_dim, rotary_dim, base=base, sections=sections,
+                             interleaved=interleaved, device=device)
+
+
+@rotary_append.register_fake
+def _(q, k, v, positions, kv_pool, slot_mapping, rotary_dim, base=10000.0, sections=None,
+      interleaved=False, q_weight=None, k_weight=None, eps=1e-6):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{_LIB}::shared_prefix_attention", mutates_args=())
+def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tensor,
+                            ctx_len: torch.Tensor, scale: float, group_rows: List[int],
+                            group_sizes: List[int], prefix_tokens: List[int],
+                            max_suffix_pages: Optional[int] = None,
+                            total_suffix_pages: Optional[int] = None) -> torch.Tensor:
+    """Decode attention of q [B, Hq, D] with shared prefixes read once; returns out. Group i
+    is the next group_sizes[i] of group_rows, sharing prefix_tokens[i] tokens (the plan is
+    laid out in every call: a program that decodes on keeps a paged.PrefixGroups)."""
+    if len(group_sizes) != len(prefix_tokens) or sum(group_sizes) != len(group_rows):
+        raise ValueError("shared_prefix_attention: group_rows, group_sizes and prefix_tokens "
+                         "do not describe the same groups")
+    groups, at = [], 0
+    for size, tokens in zip(group_sizes, prefix_tokens):
+        groups.append((group_rows[at:at + size], tokens))
+        at += size
+    plan = paged.PrefixGroups(groups, q.shape[0], q.shape[1], kv_pool.shape[1], q.shape[2],
+                              device=q.device)
+    return paged.shared_prefix_attention(q, kv_pool, block_table, ctx_len, scale, plan,
+                                         max_suffix_pages=max_suffix_pages,
+                                         total_suffix_pages=total_suffix_pages)
+
+
+@shared_prefix_attention.register_fake
+def _(q, kv_pool, block_table, ctx_len, scale, group_rows, group_sizes, prefix_tokens,
+      max_suffix_pages=None, total_suffix_pages=None):
+    return torch.empty_like(q)
+
+
+@torch.library.custom_op(f"{_LIB}::beam_select", mutates_args=())
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int,
+                finished: Optional[torch.Tensor] = None, pad_token: int = 0
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The n best continuations of each group's beams: (scores, parents, tokens) [G, n]."""
+    best, parents, tokens = beam.beam_select(logits, scores, n, finished=finished,
+                                             pad_token=pad_token)
+    return best, parents.clone(), tokens.clone()  # an operator's results share no storage
+
+
+@beam_select.register_fake
+def _(logits, scores, n, finished=None, pad_token=0):
+    shape = (logits.shape[0], n)
+    return (scores.new_empty(shape, dtype=torch.float32),
+            scores.new_empty(shape, dtype=torch.int32), scores.new_empty(shape, dtype=torch.int32))
+
+
+@torch.library.custom_op(f"{_LIB}::reorder_rows", mutates_args=("pools",))
+def reorder_rows(pools: List[torch.Tensor], slots: torch.Tensor, parents: torch.Tensor
+                 ) -> torch.Tensor:
+    """Rows of every pool follow their beams, in place; returns the new slots."""
+    return beam.reorder_rows(pools, slots, parents)
+
+
+@reorder_rows.register_fake
+def _(pools, slots, parents):
+    return torch.empty_like(slots)
+
+
+GROUP_OPERATORS = ("rotary_append", "shared_prefix_attention", "beam_select", "reorder_rows")
