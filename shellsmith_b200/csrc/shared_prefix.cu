@@ -193,6 +193,8 @@ __global__ void __maxnreg__(112)
     mbar_init(qfull, kSoftThreads);
     fence_mbar_init();
   }
+  if (warp == kMmaWarp) tc::tmem_alloc(s_tmem, 512);
+  tc::fence_before();
   pdl_wait();
   if (tid == 0 && blockIdx.x + blockIdx.y + blockIdx.z == 0) {
     // The tail starts once every CTA has triggered; its counters are zero by then.
@@ -200,41 +202,67 @@ __global__ void __maxnreg__(112)
     __threadfence();
   }
   __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *s_tmem;
   pdl_trigger();
 
   const int4 tile = a.tiles[blockIdx.z];
   const int p0 = split * a.pages_per_split;
-  if (p0 >= tile.z) return;  // uniform over the CTA
-  if (smem_addr(sm) & 1023u) {  // never seen; better void than wrong
-    if (tid == 0) flag_device(a.status, DEV_WAIT_TIMEOUT);
+  const bool misplaced = (smem_addr(sm) & 1023u) != 0;  // never seen; better void than wrong
+  const bool bad =
+      tile.w < 0 || tile.w >= a.B || tile.z > a.max_pages || tile.y * a.G > kRowsTile;
+  if (p0 >= tile.z || misplaced || bad) {  // uniform over the CTA
+    if (tid == 0 && p0 < tile.z)
+      flag_device(a.status, bad ? DEV_BAD_INDEX : DEV_WAIT_TIMEOUT);
+    if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
     return;
   }
-  if (tile.w < 0 || tile.w >= a.B || tile.z > a.max_pages || tile.y * a.G > kRowsTile) {
-    if (tid == 0) flag_device(a.status, DEV_BAD_INDEX);
-    return;
-  }
+  // What the first tile needs is ordered before the contexts are looked at. The softmax
+  // warps read 16 rows of q each, a row by neighbouring lanes; the copy warps the ids of
+  // the first tile's pages.
+  constexpr int kChunks = D / 8, kRowsAtOnce = 32 / kChunks;  // 16-byte chunks of a row
+  const auto row_of = [&](int r) {  // row r of the tile: its row of q, -1: none
+    const int member = r / a.G, b = member < tile.y ? a.members[tile.x + member] : -1;
+    return b >= 0 && b < a.B ? b * a.Hq + kvh * a.G + (r - member * a.G) : -1;
+  };
   // A member attends here to the whole pages of its context; a page that its context
   // ends in is its tail's. Pages that no member attends to are not read.
   const auto pages_of = [&](int b) { return min(tile.z, max(a.ctx_len[b], 0) / kPageTok); };
+  int reach = 0;
   if (tid < tile.y) {
     const int b = a.members[tile.x + tid];
     if (b >= 0 && b < a.B)
-      atomicMax(&s_pages, pages_of(b));
+      reach = pages_of(b);
     else
       flag_device(a.status, DEV_BAD_INDEX);
   }
+  uint4 q[kChunks / 2];
+  int first_page = 0;
+  const int which = warp == kTmaWarp ? 0 : 1;  // of the copy warps: K (half pages), V (pages)
+  const int pg = which ? lane : lane >> 1;
+  const int32_t* table = a.block_table + (size_t)tile.w * a.max_pages + p0;
+  if (warp < kTmaWarp) {
+    const int mine = lane < 16 ? row_of(16 * warp + lane) : -1;
+#pragma unroll
+    for (int j = 0; j < kChunks / 2; ++j) {
+      const int from = __shfl_sync(0xffffffffu, mine, j * kRowsAtOnce + lane / kChunks);
+      q[j] = from < 0 ? make_uint4(0u, 0u, 0u, 0u)
+                      : reinterpret_cast<const uint4*>(a.q)[(size_t)from * kChunks + lane % kChunks];
+    }
+  } else if (warp < kMmaWarp && pg < S::PAGES && p0 + pg < tile.z) {
+    first_page = table[pg];
+  }
+  if (reach > 0) atomicMax(&s_pages, reach);
   const bool stop = a.status != nullptr &&
                     (*reinterpret_cast<volatile unsigned int*>(a.status) & DEV_WAIT_TIMEOUT);
   // After a bounded wait has given up on this device, later CTAs stop at once.
-  if (__syncthreads_or(stop)) return;
+  const bool stopped = __syncthreads_or(stop);
   const int npages = min(p0 + a.pages_per_split, s_pages) - p0;
-  if (npages <= 0) return;
+  if (stopped || npages <= 0) {
+    if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+    return;
+  }
   const int ntiles = (npages + S::PAGES - 1) / S::PAGES;
-  if (warp == kMmaWarp) tc::tmem_alloc(s_tmem, 512);
-  tc::fence_before();
-  __syncthreads();
-  tc::fence_after();
-  const uint32_t tmem = *s_tmem;
 
   // Every wait is bounded. After one has given up (the status word says so) a role runs
   // on without waiting, so that the others' barriers still complete; the results are void.
@@ -246,18 +274,18 @@ __global__ void __maxnreg__(112)
   if (warp == kTmaWarp || warp == kTmaWarp + 1) {
     // ---------------------------------------------------------------- TMA
     // One box a lane: half pages of K, pages of V.
-    const int which = warp - kTmaWarp;
-    const int32_t* row = a.block_table + (size_t)tile.w * a.max_pages + p0;
     const int boxes = which ? S::PAGES : 2 * S::PAGES;
     const int box_bytes = which ? S::PAGE_BYTES : S::PAGE_BYTES / 2;
-    const int pg = which ? lane : lane >> 1;
     const bool moves = lane < boxes;
     uint64_t *full = which ? vfull : kfull, *freed = which ? vfree : kfree;
     const CUtensorMap* map = which ? &whole_pages : &half_pages;
     const auto page_of = [&](int i) {  // pages past the end repeat the last one (masked)
-      return moves && i < ntiles ? row[min(i * S::PAGES + pg, npages - 1)] : 0;
+      return moves && i < ntiles ? table[min(i * S::PAGES + pg, npages - 1)] : 0;
     };
-    int page = page_of(0);
+    const int last = npages - 1;
+    int page = __shfl_sync(0xffffffffu, first_page, min(pg, last) * (which ? 1 : 2) & 31);
+    if (!moves) page = 0;
+    if (which) wait(qfull, 0);  // q lies where V goes
     for (int i = 0; i < ntiles; ++i) {
       const int next = page_of(i + 1);
       const int st = i % S::STAGES, round = i / S::STAGES;
@@ -331,26 +359,33 @@ __global__ void __maxnreg__(112)
     constexpr int kOut = D / 2;         // and of O and Q
     const int half = warp >> 2, r = tid & (kRowsTile - 1);
     const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's TMEM lanes
-    const int member = r / a.G, h = r - member * a.G;
-    const int b = member < tile.y ? a.members[tile.x + member] : -1;
-    const bool live = b >= 0 && b < a.B;
+    const int out_row = row_of(r);
+    const bool live = out_row >= 0;
     const bool idle = !__any_sync(0xffffffffu, live);  // no row here: only the barriers
-    const size_t out_row = live ? (size_t)b * a.Hq + kvh * a.G + h : 0;
     // Pages of this split that the row attends to (its context may end inside the prefix).
-    const int limit = live ? min(pages_of(b) - p0, npages) : 0;
+    const int limit = live ? min(pages_of(out_row / a.Hq) - p0, npages) : 0;
     // A negative scale turns q, so that the largest score stays the largest; a zero one
     // clears it.
     const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
     const uint32_t keep = a.scale_log2 == 0.f || !live ? 0u : 0xffffffffu;
     const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
     {
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + out_row * D + half * kOut);
+      // q turns from a row by 8 to 32 lanes to a row a lane in the V stages, whose copies
+      // wait for it; chunk c of row r at c ^ r keeps both ways free of bank conflicts.
+      uint8_t* turn = sm + S::STAGES * S::TILE_BYTES;
+      const auto chunk = [&](int row, int c) {
+        return reinterpret_cast<uint4*>(turn + row * (D * 2) + ((c ^ (row & (kChunks - 1))) * 16));
+      };
+#pragma unroll
+      for (int j = 0; j < kChunks / 2; ++j)
+        *chunk(16 * warp + j * kRowsAtOnce + lane / kChunks, lane % kChunks) = q[j];
+      soft_sync();
 #pragma unroll
       for (int c = 0; c < kOut / 32; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const uint4 u = src[4 * c + x];
+          const uint4 u = *chunk(r, half * (kChunks / 2) + 4 * c + x);
           w[4 * x] = u.x;
           w[4 * x + 1] = u.y;
           w[4 * x + 2] = u.z;
@@ -360,6 +395,7 @@ __global__ void __maxnreg__(112)
         for (int x = 0; x < 16; ++x) w[x] = (w[x] ^ flip) & keep;
         tc::tmem_st16(mine + S::T_Q + half * (kOut / 2) + 16 * c, w);
       }
+      fence_proxy_async_smem();
       tc::tmem_wait_st();
       tc::fence_before();
       mbar_arrive(qfull);
@@ -440,32 +476,39 @@ __global__ void __maxnreg__(112)
     soft_sync();
     l += s_half[half ^ 1][r];
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    const size_t part = out_row * a.num_splits + split;
-    // Each thread stages its half row in the stages, which no copy or product uses any
-    // more, and sends it off as bulk copies: a row is contiguous in global memory.
-    uint8_t* stage = sm + tid * S::PITCH;
+    // The parts leave through the stages, which no copy or product uses any more: a piece
+    // of the warp's 32 rows, a row a lane, then a row by neighbouring lanes.
+    constexpr int kLanes = S::PIECE / 4, kRowsOut = 32 / kLanes;  // of a row, of a store
+    uint8_t* stage = sm + warp * 32 * S::PITCH;
+    if (!idle && __all_sync(0xffffffffu, ok)) {
 #pragma unroll 1
-    for (int c = 0; c < kOut; c += S::PIECE) {
-      if (c > 0) bulk_wait_read_all();
+      for (int c = 0; c < kOut; c += S::PIECE) {
 #pragma unroll
-      for (int p = 0; p < S::PIECE / 32; ++p) {
-        float o[32];
-        tc::tmem_ld32(mine + half * kOut + c + 32 * p, o);
+        for (int p = 0; p < S::PIECE / 32; ++p) {
+          float o[32];
+          tc::tmem_ld32(mine + half * kOut + c + 32 * p, o);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          reinterpret_cast<float4*>(stage + 128 * p)[e] = make_float4(
-              o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv);
-      }
-      fence_proxy_async_smem();
-      if (live && ok) {
-        bulk_s2g(a.part_out + part * D + half * kOut + c, stage, S::PIECE * 4);
-        bulk_commit();
+          for (int e = 0; e < 8; ++e)
+            reinterpret_cast<float4*>(stage + lane * S::PITCH + 128 * p)[e] = make_float4(
+                o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv);
+        }
+        __syncwarp();
+#pragma unroll 8
+        for (int i = 0; i < kLanes; ++i) {
+          const int from = i * kRowsOut + lane / kLanes, col = lane % kLanes;
+          const int to = __shfl_sync(0xffffffffu, out_row, from);
+          const float4 v = reinterpret_cast<const float4*>(stage + from * S::PITCH)[col];
+          if (to >= 0)
+            reinterpret_cast<float4*>(a.part_out + ((size_t)to * a.num_splits + split) * D +
+                                      half * kOut + c)[col] = v;
+        }
+        __syncwarp();
       }
     }
     if (live && half == 0)
-      a.part_lse[part] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f
-                                 : (l == 0.f ? -CUDART_INF_F : l);  // a NaN stays one
-    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the parts are written
+      a.part_lse[(size_t)out_row * a.num_splits + split] =
+          l > 0.f ? (m + log2f(l)) * 0.6931471805599453f
+                  : (l == 0.f ? -CUDART_INF_F : l);  // a NaN stays one
   }
   __syncwarp();
   tc::fence_before();
