@@ -79,10 +79,26 @@ template <>
 struct Logits<uint16_t> {  // bf16
   static constexpr int kPerVec = 8;
   static constexpr int kBits = 16;  // significant high bits of a key
-  __device__ static float largest(const uint4& u) {  // NaN only where all are
+  using Top = __nv_bfloat162;  // the maxima of a granule's even and odd logits
+  __device__ static Top tops(const uint4& u) {  // NaN only where all are
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  }
+  __device__ static Top join_tops(Top a, Top b) { return __hmax2(a, b); }
+  __device__ static float largest(Top t) { return fmaxf(__low2float(t), __high2float(t)); }
+  // x + shift of a pair of logits, in fp32.
+  __device__ static uint64_t shifted(const uint4& u, int e, float shift) {
+    const uint32_t w = e < 2 ? u.x : e < 4 ? u.y : e < 6 ? u.z : u.w;
+    float lo, hi;
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "mov.b32 {a, b}, %2;\n\t"
+        "add.rn.f32.bf16 %0, a, %3;\n\t"
+        "add.rn.f32.bf16 %1, b, %3;\n\t}"
+        : "=f"(lo), "=f"(hi)
+        : "r"(w), "f"(shift));
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+    return p;
   }
   __device__ static float value(uint16_t x) { return bf16_to_f(x); }
   __device__ static float get(const uint4& u, int e) {
@@ -105,8 +121,21 @@ template <>
 struct Logits<float> {
   static constexpr int kPerVec = 4;
   static constexpr int kBits = 32;
-  __device__ static float largest(const uint4& u) {
+  using Top = float;
+  __device__ static Top tops(const uint4& u) {
     return fmaxf(fmaxf(get(u, 0), get(u, 1)), fmaxf(get(u, 2), get(u, 3)));
+  }
+  __device__ static Top join_tops(Top a, Top b) { return fmaxf(a, b); }
+  __device__ static float largest(Top t) { return t; }
+  __device__ static uint64_t shifted(const uint4& u, int e, float shift) {
+    uint64_t p;
+    asm("{\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %2};\n\t"
+        "mov.b64 b, {%3, %3};\n\t"
+        "add.rn.f32x2 %0, a, b;\n\t}"
+        : "=l"(p)
+        : "f"(get(u, e)), "f"(get(u, e + 1)), "f"(shift));
+    return p;
   }
   __device__ static float value(float x) { return x; }
   __device__ static float get(const uint4& u, int e) {
@@ -376,12 +405,13 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const SelectArgs 
 #pragma unroll 1
   for (; g0 - lane < g_end; g0 += kRound) {
     load(g0 + kRound, next);
-    float top[kVecs];
+    typename L::Top tops[kVecs];
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) top[j] = L::largest(r[j]);
-    float all = top[0];
-#pragma unroll
-    for (int j = 1; j < kVecs; ++j) all = fmaxf(all, top[j]);
+    for (int j = 0; j < kVecs; ++j) tops[j] = L::tops(r[j]);
+    const float all = L::largest(L::join_tops(L::join_tops(tops[0], tops[1]),
+                                              L::join_tops(tops[2], tops[3])));
+    static_assert(kVecs == 4, "joined above");
+    const auto top = [&](int j) { return L::largest(tops[j]); };
     if (all > m) {
       s *= m == -CUDART_INF_F ? 1.f : ex2((m - all) * kLog2e);  // a NaN sum stays
       m = all;
@@ -393,9 +423,7 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const SelectArgs 
 #pragma unroll
       for (int e = 0; e < E; e += 2) {
         float y0, y1;
-        unpair(mul2(add2(pair(L::get(r[j], e), L::get(r[j], e + 1)), pair(shift, shift)),
-                    pair(kLog2e, kLog2e)),
-               y0, y1);
+        unpair(mul2(L::shifted(r[j], e, shift), pair(kLog2e, kLog2e)), y0, y1);
         sums[e / 2 % 2] = add2(sums[e / 2 % 2], pair(ex2(y0), ex2(y1)));
       }
     float s0, s1;
@@ -407,13 +435,13 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const SelectArgs 
       const float least = least_k == 0u ? -CUDART_INF_F : L::unkey(least_k);
       if (__any_sync(kAll, all > own && all >= least)) {
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j) hot |= (top[j] > own && top[j] >= least) ? 1u << j : 0u;
+        for (int j = 0; j < kVecs; ++j) hot |= (top(j) > own && top(j) >= least) ? 1u << j : 0u;
       }
     } else {
       first = false;
       uint32_t k[kVecs];
 #pragma unroll
-      for (int j = 0; j < kVecs; ++j) k[j] = L::key(top[j]);
+      for (int j = 0; j < kVecs; ++j) k[j] = L::key(top(j));
       const uint32_t t = warp_nth<kVecs>(k, want);
       if (t != 0u) own = L::unkey(t);
       if (lane == 0) atomicMax(&shared_bound, t);
@@ -435,7 +463,7 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const SelectArgs 
             if (at < kGranules) {  // an overflow is seen at the end
               gran[at] = r[j];
               gran_v[at] = (g0 + 32 * j) * E - lead;
-              gran_k[at] = L::key(top[j]);
+              gran_k[at] = L::key(top(j));
             }
             ++at;
           }
