@@ -34,6 +34,13 @@
 // are at most its last kept one t, and one equal to t has a higher index; if the next
 // value below t still scores as much as the n-th best, merge_kernel rescans the group's
 // logits for scores equal to it, in index order, until it has enough.
+//
+// Measured (B200): 32 groups of 8 beams over 250,001 bf16 tokens, a fifth of the rows
+// finished (106 MB), 38.5 us, 2.8 TB/s: the scan's 18.6 million warp instructions fill 60 %
+// of the issue slots and its exponentials 43 % of their unit, while DRAM is 39 % busy. Its
+// time is arithmetic and the chains in it, not memory: three bulk-copied blocks a warp in
+// flight instead of the one in registers took 43.2 us. 8 groups of 5 over 50,001 fp32
+// tokens 14.1 us, 1 of 4 over 32,768 10.2 us: two launches, a block's bound and the merge.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -49,7 +56,8 @@ constexpr int kMaxSelect = 64;       // n
 constexpr int kScanWarps = kScanThreads / 32;
 constexpr int kVecs = 4;             // 16-byte loads of a lane per block
 constexpr int kScanList = kMaxSelect + 1 + kScanThreads * 8 + 63;  // n + 1 and a load a lane
-constexpr int kSegWaves = 4;         // segments per SM, all resident
+// Segments per SM: the case of 256 rows above took 38.5 us with 4, 48 with 2 and 47 with 8.
+constexpr int kSegWaves = 4;
 constexpr int kGranules = 512;       // listed granules
 constexpr int kNewest = 128;         // list entries that make a bound
 constexpr int kRankList = 256;       // lists up to here are ranked in one go
@@ -337,6 +345,7 @@ __device__ __noinline__ int ordered_list(const T* base, int lead, int V, int g_b
   return *n_list;
 }
 
+// Three CTAs an SM: the case of 256 rows above took 38.5 us, with four (64 registers) 44.8.
 template <typename T>
 __global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const SelectArgs a) {
   using L = Logits<T>;
@@ -468,7 +477,8 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const SelectArgs 
             ++at;
           }
       }
-      // Has the list grown enough for a better bound, and is it this warp that makes it?
+      // Has the list grown enough for a better bound, and is it this warp that makes it? (Every
+      // n + 1 entries; every 2 (n + 1): 39.5 us instead of 38.4.)
       int now = 0;
       if (lane == 0) {
         now = *reinterpret_cast<volatile int*>(&n_gran);

@@ -21,6 +21,13 @@
 // values each as two 4-value pieces: a lane of the rotary part holds both halves of four
 // pairs, so that a turn needs no exchange, and the norm is a shuffle sum. Products go two
 // at a time (fp32 pairs).
+//
+// Measured (B200, 16 + 2 + 2 heads of 256, three axes, 64 rotary dims): 16,381 tokens
+// (336 MB) 64 us, 5.2 TB/s, 79 % of a plain copy's rate: half of the issue slots are busy
+// and the writes to the pool's pages leave in pieces of a row; 85 us before the rows of a
+// head were walked by one warp and products paired. 8 tokens 3.0 us, 256 tokens of 24 + 8 +
+// 8 heads of 128 4.0 us: a launch, the table and one row. Operands off a 16-byte boundary (or strides that are)
+// are read by the element: 256 tokens 5.5 us against 5.0 beside it, 16,381 85 against 63.
 #include <algorithm>
 #include <type_traits>
 
