@@ -63,6 +63,7 @@ constexpr int kNewest = 128;         // list entries that make a bound
 constexpr int kRankList = 256;       // lists up to here are ranked in one go
 constexpr int kMergeCache = 4096;    // candidates whose keys merge_kernel keeps
 constexpr int kMergeList = 1024;
+constexpr int kMergeAhead = 4;       // items of a thread that are loaded at once
 constexpr int kMaxBeams = 64;
 
 // Order-preserving unsigned keys of finite values and +inf; 0 for -inf and NaN.
@@ -367,14 +368,6 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const SelectArgs 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.y, want = a.n + 1;
   const size_t seg = (size_t)row * a.segs + blockIdx.x;
-  if (row_idle(a, row)) return;  // uniform over the CTA; merge_kernel skips the row too
-  for (int i = tid; i < kGranules; i += kScanThreads) gran_k[i] = 0u;  // 0: not written yet
-  if (tid == 0) {
-    shared_bound = 0u;
-    n_gran = n_list = 0;
-    refresh_at = 2 * want;
-  }
-  __syncthreads();
   // Aligned 16-byte granules over the row; the first and the last may hold elements
   // outside it, which are read one by one.
   const T* base = reinterpret_cast<const T*>(a.logits) + (long long)row * a.row_stride;
@@ -402,15 +395,23 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const SelectArgs 
       }
     }
   };
+  constexpr int kRound = kScanWarps * kBlock;
+  uint4 r[kVecs], next[kVecs];
+  load(g0, r);  // before the row's flags are known, which takes as long
+  if (row_idle(a, row)) return;  // uniform over the CTA; merge_kernel skips the row too
+  for (int i = tid; i < kGranules; i += kScanThreads) gran_k[i] = 0u;  // 0: not written yet
+  if (tid == 0) {
+    shared_bound = 0u;
+    n_gran = n_list = 0;
+    refresh_at = 2 * want;
+  }
+  __syncthreads();
   // This lane's maximum and the sum of e^(x - m). x - m comes before the change of base: a
   // product with log2 e would add its rounding to the largest terms (and overflow at the
   // type's ends).
   float m = -CUDART_INF_F, s = 0.f;
   float own = -CUDART_INF_F;  // this warp's first bound: later granules count above it
   bool first = true;
-  constexpr int kRound = kScanWarps * kBlock;
-  uint4 r[kVecs], next[kVecs];
-  load(g0, r);
 #pragma unroll 1
   for (; g0 - lane < g_end; g0 += kRound) {
     load(g0 + kRound, next);
@@ -588,15 +589,32 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const SelectArgs a
   pdl_trigger();
   const int g = blockIdx.x, K = a.K, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) n_list = ambiguous = strictly = 0, last_score = 0u;
+  // Items: the segments' candidates, then one per beam for the finished ones. A thread's
+  // first ones and its first floor are loaded beside the rows' statistics; those of an idle
+  // row are not used.
+  const int per = a.n + 1, segs = K * a.segs, cands = segs * per, items = cands + K;
+  const uint2* kept = a.kept + (size_t)g * cands;
+  const float* floors = a.floors + (size_t)g * segs;
+  uint2 ahead[kMergeAhead];
+#pragma unroll
+  for (int x = 0; x < kMergeAhead; ++x) {
+    const int i = threadIdx.x + x * kMergeThreads;
+    ahead[x] = i < cands ? kept[i] : make_uint2(0u, 0u);
+  }
+  const float floor_ahead = (int)threadIdx.x < segs ? floors[threadIdx.x] : 0.f;
   for (int k = warp; k < K; k += kMergeThreads / 32) {
     const int row = g * K + k;
     float m = -CUDART_INF_F, s = 0.f;
+    const float2* stats = a.stats + (size_t)row * a.segs;
+    const float2 st0 = lane < a.segs ? stats[lane] : make_float2(m, s);
     const bool on = !row_idle(a, row);
-    if (on)
-      for (int c = lane; c < a.segs; c += 32) {
-        const float2 st = a.stats[(size_t)row * a.segs + c];
+    if (on) {
+      join(m, s, st0.x, st0.y);
+      for (int c = lane + 32; c < a.segs; c += 32) {
+        const float2 st = stats[c];
         join(m, s, st.x, st.y);
       }
+    }
     warp_join(m, s);
     if (lane == 0) {
       row_m[k] = m;
@@ -613,26 +631,29 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const SelectArgs a
     return key == 0u ? 0ull
                      : ((unsigned long long)key << 32) | (0xffffffffu - ((uint32_t)k * a.V + v));
   };
-  // Items: the segments' candidates, then one per beam for the finished ones.
-  const int per = a.n + 1, segs = K * a.segs, cands = segs * per, items = cands + K;
-  const auto make = [&](int i) -> unsigned long long {
+  const auto keyed = [&](int i, uint2 c) -> unsigned long long {
     if (i >= cands) {
       const int k = i - cands;
       const bool fin = a.finished != nullptr && a.finished[g * K + k];
       return fin ? full_key(k, row_s[k], a.pad) : 0ull;
     }
     const int k = i / (a.segs * per);
-    if (!row_on[k]) return 0ull;
-    const uint2 c = a.kept[(size_t)g * cands + i];
-    return full_key(k, score(k, __uint_as_float(c.x)), (int)c.y);
+    return row_on[k] ? full_key(k, score(k, __uint_as_float(c.x)), (int)c.y) : 0ull;
   };
+  const auto make = [&](int i) { return keyed(i, i < cands ? kept[i] : make_uint2(0u, 0u)); };
   const bool cached = items <= kMergeCache;
   unsigned long long best = 0ull;
-  for (int i = threadIdx.x; i < items; i += kMergeThreads) {
-    const unsigned long long key = make(i);
+  const auto see = [&](int i, unsigned long long key) {
     if (cached) cache[i] = key;
     best = key > best ? key : best;
+  };
+#pragma unroll
+  for (int x = 0; x < kMergeAhead; ++x) {
+    const int i = threadIdx.x + x * kMergeThreads;
+    if (i < items) see(i, keyed(i, ahead[x]));
   }
+  for (int i = threadIdx.x + kMergeAhead * kMergeThreads; i < items; i += kMergeThreads)
+    see(i, make(i));
   const auto item = [&](int i) { return cached ? cache[i] : make(i); };  // own items only
   // At least n items reach about the n-th largest of the threads' best scores.
   best_k[threadIdx.x] = (uint32_t)(best >> 32);
@@ -707,7 +728,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const SelectArgs a
   for (int sgm = threadIdx.x; sgm < segs; sgm += kMergeThreads) {
     const int k = sgm / a.segs;
     if (!row_on[k]) continue;
-    const float fl = a.floors[(size_t)g * segs + sgm];
+    const float fl = sgm < kMergeThreads ? floor_ahead : floors[sgm];
     if (fl > -CUDART_INF_F && score_key(score(k, L::below(fl))) >= last) ambiguous = 1;
   }
   for (int i = threadIdx.x; i < total; i += kMergeThreads)
