@@ -40,7 +40,7 @@
 // of the issue slots and its exponentials 43 % of their unit, while DRAM is 39 % busy. Its
 // time is arithmetic and the chains in it, not memory: three bulk-copied blocks a warp in
 // flight instead of the one in registers took 43.2 us. 8 groups of 5 over 50,001 fp32
-// tokens 14.1 us, 1 of 4 over 32,768 10.2 us: two launches, a block's bound and the merge.
+// tokens 14.1 us, 1 of 4 over 32,768 9.9 us: two launches, a block's bound and the merge.
 #include <math_constants.h>
 
 #include <algorithm>

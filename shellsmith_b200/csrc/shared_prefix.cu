@@ -43,13 +43,13 @@
 //
 // Measured (B200, 16 query over 2 kv heads of 256 unless said):
 //   8 groups of 8 sequences, prefixes of 16,272 and tails of U[1, 2048] tokens (402 MB)
-//     73.9 us, 5.4 TB/s, 83 % of a plain copy's rate: HBM, but for 5 us of start and 8 of
+//     74.2 us, 5.4 TB/s, 83 % of a plain copy's rate: HBM, but for 5 us of start and 8 of
 //     the last CTAs' parts and the merge
 //   128 sequences on 8,208 tokens, tails of U[1, 1024] (153 MB) 47.9 us: the prefix's eight
 //     tiles read it from the L2 and their products, the tails' loads and both softmaxes
 //     share the SMs for 40 us; the tails alone take 35
-//   3 groups of 5 on 5,104, tails of U[1, 777], 24 over 8 heads of 128 (87 MB) 24.1 us
-//   8 on 2,048, tails of U[1, 64] (5 MB) 12.3 us: the chain of three kernels (8 + 4 us)
+//   3 groups of 5 on 5,104, tails of U[1, 777], 24 over 8 heads of 128 (87 MB) 24.3 us
+//   8 on 2,048, tails of U[1, 64] (5 MB) 12.4 us: the chain of three kernels (8 + 4 us)
 #include <cudaTypedefs.h>
 #include <math_constants.h>
 
@@ -222,9 +222,11 @@ __global__ void __maxnreg__(112)
     mbar_init(qfull, kSoftThreads);
     fence_mbar_init();
   }
+  // All of TMEM, taken after the wait (a CTA of the kernel before this one might still have
+  // to take its own) and before this kernel's dependents may start.
+  pdl_wait();
   if (warp == kMmaWarp) tc::tmem_alloc(s_tmem, 512);
   tc::fence_before();
-  pdl_wait();
   if (tid == 0 && blockIdx.x + blockIdx.y + blockIdx.z == 0) {
     // The tail starts once every CTA has triggered; its counters are zero by then.
     for (int i = 0; i < a.slabs; ++i) atomicExch(a.counters + i, 0);
