@@ -43,13 +43,13 @@
 //
 // Measured (B200, 16 query over 2 kv heads of 256 unless said):
 //   8 groups of 8 sequences, prefixes of 16,272 and tails of U[1, 2048] tokens (402 MB)
-//     74.2 us, 5.4 TB/s, 83 % of a plain copy's rate: HBM, but for 5 us of start and 8 of
+//     73.5 us, 5.5 TB/s, 83 % of a plain copy's rate: HBM, but for 5 us of start and 8 of
 //     the last CTAs' parts and the merge
-//   128 sequences on 8,208 tokens, tails of U[1, 1024] (153 MB) 47.9 us: the prefix's eight
+//   128 sequences on 8,208 tokens, tails of U[1, 1024] (153 MB) 47.8 us: the prefix's eight
 //     tiles read it from the L2 and their products, the tails' loads and both softmaxes
 //     share the SMs for 40 us; the tails alone take 35
-//   3 groups of 5 on 5,104, tails of U[1, 777], 24 over 8 heads of 128 (87 MB) 24.3 us
-//   8 on 2,048, tails of U[1, 64] (5 MB) 12.4 us: the chain of three kernels (8 + 4 us)
+//   3 groups of 5 on 5,104, tails of U[1, 777], 24 over 8 heads of 128 (87 MB) 24.0 us
+//   8 on 2,048, tails of U[1, 64] (5 MB) 12.3 us: the chain of three kernels (8 + 4 us)
 #include <cudaTypedefs.h>
 #include <math_constants.h>
 
@@ -222,19 +222,13 @@ __global__ void __maxnreg__(112)
     mbar_init(qfull, kSoftThreads);
     fence_mbar_init();
   }
-  // All of TMEM, taken after the wait (a CTA of the kernel before this one might still have
-  // to take its own) and before this kernel's dependents may start.
   pdl_wait();
-  if (warp == kMmaWarp) tc::tmem_alloc(s_tmem, 512);
-  tc::fence_before();
   if (tid == 0 && blockIdx.x + blockIdx.y + blockIdx.z == 0) {
     // The tail starts once every CTA has triggered; its counters are zero by then.
     for (int i = 0; i < a.slabs; ++i) atomicExch(a.counters + i, 0);
     __threadfence();
   }
   __syncthreads();
-  tc::fence_after();
-  const uint32_t tmem = *s_tmem;
   pdl_trigger();
 
   const int4 tile = a.tiles[blockIdx.z];
@@ -245,9 +239,12 @@ __global__ void __maxnreg__(112)
   if (p0 >= tile.z || misplaced || bad) {  // uniform over the CTA
     if (tid == 0 && p0 < tile.z)
       flag_device(a.status, bad ? DEV_BAD_INDEX : DEV_WAIT_TIMEOUT);
-    if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
     return;
   }
+  // All of TMEM, while the others load: after the wait (a CTA of the kernel before this one
+  // might still have had to take its own); the kernels that start beside this one use none.
+  if (warp == kMmaWarp) tc::tmem_alloc(s_tmem, 512);
+  tc::fence_before();
   // What the first tile needs is ordered before the contexts are looked at. The softmax
   // warps read 16 rows of q each, a row by neighbouring lanes; the copy warps the ids of
   // the first tile's pages.
@@ -288,6 +285,8 @@ __global__ void __maxnreg__(112)
                     (*reinterpret_cast<volatile unsigned int*>(a.status) & DEV_WAIT_TIMEOUT);
   // After a bounded wait has given up on this device, later CTAs stop at once.
   const bool stopped = __syncthreads_or(stop);
+  tc::fence_after();
+  const uint32_t tmem = *s_tmem;
   const int npages = min(p0 + a.pages_per_split, s_pages) - p0;
   if (stopped || npages <= 0) {
     if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
