@@ -328,8 +328,11 @@ __device__ __noinline__ int ordered_list(const T* base, int lead, int V, int g_b
     for (int e = 0; e < E; ++e)
       k[e] = g0 + (int)threadIdx.x < g_end && v0 + e >= 0 && v0 + e < V ? L::key(L::value(base[v0 + e]))
                                                                        : 0u;
-    if (*n_list > 2 * want) {  // uniform
-      const int total = *n_list;
+    // Every thread has read the count before one appends: the branch holds barriers, and a
+    // warp that came late would see what the early ones appended.
+    const int total = *n_list;
+    __syncthreads();
+    if (total > 2 * want) {  // uniform
       bound = max(bound, cut_list<L::kBits>(list_k, list_v, total, want, scratch));
       if (threadIdx.x == 0) *n_list = want;
       __syncthreads();
