@@ -55,7 +55,9 @@ constexpr int kMergeThreads = 256;
 constexpr int kMaxSelect = 64;       // n
 constexpr int kScanWarps = kScanThreads / 32;
 constexpr int kVecs = 4;             // 16-byte loads of a lane per block
-constexpr int kScanList = kMaxSelect + 1 + kScanThreads * 8 + 63;  // n + 1 and a load a lane
+// Candidates of a segment. ordered_list leaves up to 2 (n + 1) before it cuts, and a tile
+// then appends up to a granule's logits (8 at most) a thread.
+constexpr int kScanList = 2 * (kMaxSelect + 1) + kScanThreads * 8;
 // Segments per SM: the case of 256 rows above took 38.5 us with 4, 48 with 2 and 47 with 8.
 constexpr int kSegWaves = 4;
 constexpr int kGranules = 512;       // listed granules
@@ -318,6 +320,7 @@ __device__ __noinline__ int ordered_list(const T* base, int lead, int V, int g_b
                                          int* n_list) {
   using L = Logits<T>;
   constexpr int E = L::kPerVec;
+  static_assert(kScanList >= 2 * (kMaxSelect + 1) + kScanThreads * E, "a tile past the last cut");
   if (threadIdx.x == 0) *n_list = 0;
   __syncthreads();
   uint32_t bound = 0u;

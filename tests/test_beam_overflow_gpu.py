@@ -56,3 +56,20 @@ def test_overflowing_lists(cuda, dtype, n, kind):
         x = _rows(kind, R, V, cuda).to(dtype)
         for _ in range(3):
             _exact(x, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("left", [129, 130, 131])
+def test_tile_after_a_list_that_is_just_not_cut(cuda, dtype, left):
+    """n = 64: a segment whose first tile (256 granules of 16 bytes) leaves 129 to 131 logits,
+    one a granule and 65 in each of the first two blocks of 128, before tiles of equal lower
+    ones. 130 entries are not cut yet, and the next tile appends a whole tile's."""
+    per = 16 // dtype.itemsize
+    V = 60 * 256 * per
+    x = torch.full((V,), 0.5, device=cuda)
+    x[:256 * per] = -float("inf")
+    block = torch.arange(128, device=cuda) * per
+    first = torch.cat([block[:65], block[:65] + 128 * per, block[65:70]])[:left]
+    x[first] = 2.0 + torch.arange(left, device=cuda) % 7 * 0.125
+    for R in (1, 5, 700):
+        _exact(x.to(dtype).expand(R, V).contiguous(), 64)
