@@ -680,6 +680,9 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
         page = 0;  // keep the copy in bounds; the status word reports the fault
       }
       const int s = issued % kTailStages;
+      // The stage may hold rows that the warp cleared with ordinary stores (a page that its
+      // context ended in); a __syncwarp stands between those and every issue.
+      fence_proxy_async_smem();
       mbar_arrive_expect_tx(&bar[s], STAGE);
       bulk_g2s_once(
           stage + s * STAGE,
@@ -790,13 +793,10 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
       }
       ++consumed;
       __syncwarp();
-      if (cur_issued < cur.n || (have_next && nxt_issued < nxt.n)) {
-        if (lane == 0) fence_proxy_async_smem();
-        if (cur_issued < cur.n)
-          issue(cur, cur_issued++);
-        else
-          issue(nxt, nxt_issued++);
-      }
+      if (cur_issued < cur.n)
+        issue(cur, cur_issued++);
+      else if (have_next && nxt_issued < nxt.n)
+        issue(nxt, nxt_issued++);
     }
     if (!ok) break;
     if (nxt.n > 0) load_q(nxt);  // arrives while the partial is written
