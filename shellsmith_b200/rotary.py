@@ -80,19 +80,18 @@ def _strides(*values) -> ctypes.Array:
 
 def _operand(name: str, t: torch.Tensor, dim: int) -> tuple:
     """Shape and strides of a [ntok, heads, D] bf16 operand."""
-    if type(t) is torch.Tensor and t.is_cuda and t.dtype is torch.bfloat16 and t.dim() == 3:
-        shape, stride = t.shape, t.stride()
-        if shape[2] == dim and (stride[2] == 1 or not t.numel()):
-            return shape, stride
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (the product path has no CPU fallback)")
-    if t.dtype != torch.bfloat16:
+    if t.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must be torch.bfloat16, got {t.dtype}")
-    if t.dim() != 3 or t.shape[2] != dim:
-        raise ValueError(f"{name} must be [ntok, heads, {dim}], got {tuple(t.shape)}")
-    raise ValueError(f"{name} must be contiguous along the head dimension")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != dim:
+        raise ValueError(f"{name} must be [ntok, heads, {dim}], got {tuple(shape)}")
+    if stride[2] != 1 and t.numel():
+        raise ValueError(f"{name} must be contiguous along the head dimension")
+    return shape, stride
 
 
 def _weight(name: str, w: torch.Tensor | None, dim: int) -> int | None:
