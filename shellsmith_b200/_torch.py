@@ -48,3 +48,11 @@ def require_cuda(name: str, t: torch.Tensor, dtype: torch.dtype, ndim: int | Non
         raise ValueError(f"{name} must be contiguous")
     if t.numel() and t.data_ptr() % align:
         raise ValueError(f"{name} must be {align}-byte aligned")
+
+
+def on_device(index: int, **operands) -> None:
+    """Refuse a CUDA operand of another GPU than `index`: a kernel that got its address would
+    fault. What is no CUDA tensor is require_cuda's to refuse."""
+    for name, t in operands.items():
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, the call on cuda:{index}")

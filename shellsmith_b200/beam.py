@@ -20,7 +20,7 @@ import numpy as np
 import torch
 
 from . import _capi
-from ._torch import fast, ptr, require_cuda, stream_of
+from ._torch import fast, on_device, ptr, require_cuda, stream_of
 
 MAX_BEAMS = 64   # beams of one group
 MAX_SELECT = 64  # continuations asked for at once
@@ -77,6 +77,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, *,
         require_cuda("finished", finished, torch.bool, 2, align=1)
         if finished.shape != (groups, beams):
             raise ValueError(f"finished must be [{groups}, {beams}], got {tuple(finished.shape)}")
+    on_device(logits.get_device(), scores=scores, finished=finished)
     need = _workspace(groups, beams, vocab, n, int(fp32))
     work = scores.new_empty(need // 4)
     best, parents, tokens = scores.new_empty((3, groups, n)).unbind(0)
@@ -121,6 +122,7 @@ def reorder_rows(pools, slots: torch.Tensor, parents: torch.Tensor) -> torch.Ten
         rows = size[1]
         bases[i], layers[i] = pool.data_ptr(), size[0]
         sizes[i] = pool.stride(1) * pool.element_size()
+    on_device(slots.get_device(), parents=parents, **{f"pool {i}": p for i, p in enumerate(pools)})
     out = torch.empty_like(slots)
     _reorder(bases, sizes, layers, count, rows or 1, slots.data_ptr(), parents.data_ptr(),
              out.data_ptr(), groups, beams or 1, stream_of(slots))

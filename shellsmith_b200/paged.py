@@ -28,7 +28,7 @@ import math
 import torch
 
 from . import _capi
-from ._torch import fast, ptr, require_cuda, stream_of
+from ._torch import fast, on_device, ptr, require_cuda, stream_of
 
 PAGE_SIZE = 16
 
@@ -518,6 +518,7 @@ class SharedPrefixWorkspace:
     def __init__(self, device: str | torch.device = "cuda"):
         self.device = torch.device(device)
         self._buffer = torch.empty(0, dtype=torch.float32, device=device)
+        self.device_index = self._buffer.get_device()
         self._floats = 0
 
     def parts(self, rows: int, dim: int, prefix_splits: int, splits: int) -> tuple:
@@ -555,6 +556,9 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
     group); when omitted the block-table width bounds them. lse_out [B * Hq] fp32. bf16
     pools only. Calls that share a workspace must not overlap on the GPU.
     """
+    if workspace is not None and workspace.device_index != groups.device_index:
+        raise ValueError(f"the workspace is on {workspace.device}, the groups on "
+                         f"{groups.tiles.device}")
     if fast is not None and workspace is not None and groups.ntiles:
         pre = groups.splits(total_suffix_pages)
         tail = tail_split_plan(groups.batch, groups.q_heads, groups.kv_heads,
@@ -580,13 +584,15 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
     max_pages = block_table.shape[1]
     if groups.max_prefix_pages > max_pages:
         raise ValueError("shared_prefix_attention: a prefix is longer than the block table")
+    if groups.device_index != q.get_device():
+        raise ValueError(f"the groups are on {groups.tiles.device}, q on {q.device}")
+    on_device(groups.device_index, kv_pool=kv_pool, block_table=block_table, ctx_len=ctx_len,
+              out=out, lse_out=lse_out)
     if groups.ntiles == 0:
         return paged_decode_attention(q, kv_pool, block_table, ctx_len, scale,
                                       max_pages_in_batch=max_suffix_pages,
                                       total_pages=total_suffix_pages, out=out, lse_out=lse_out,
                                       sms=sms)
-    if groups.device_index != q.get_device():
-        raise ValueError(f"the groups are on {groups.tiles.device}, q on {q.device}")
     pps, nsplit = tail_split_plan(B, hq, hkv, max_suffix_pages or max_pages, pages_per_split,
                                   total_suffix_pages, sms or groups.sms)
     pre_pps, pre_splits = groups.splits(total_suffix_pages)

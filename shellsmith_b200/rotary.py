@@ -20,7 +20,7 @@ import math
 import torch
 
 from . import _capi, paged
-from ._torch import fast, require_cuda, stream_of
+from ._torch import fast, on_device, require_cuda, stream_of
 
 
 class RotaryPlan:
@@ -117,6 +117,7 @@ def _run(q, k, v, k_shape, strides, positions, plan, q_weight, k_weight, eps, q_
                          f"got {positions.dtype} {tuple(positions.shape)}")
     if plan.device_index != q.get_device():
         raise ValueError(f"the plan is on {plan.turns.device}, q on {q.device}")
+    on_device(plan.device_index, k=k, positions=positions, q_weight=q_weight, k_weight=k_weight)
     _append(q.data_ptr(), k.data_ptr(), v, _strides(*strides), positions.data_ptr(), pos_stride[0],
             plan.axes, plan.turns_ptr, plan.axis_ptr, _weight("q_weight", q_weight, dim),
             _weight("k_weight", k_weight, dim), eps, q_out.data_ptr(), k_out, pool, slots, ntok,
@@ -163,6 +164,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     require_cuda("slot_mapping", slot_mapping, torch.int64, 1, align=8)
     if k_shape[1] != hkv or k_shape[2] != dim or slot_mapping.shape[0] != k_shape[0]:
         raise ValueError("rotary_append: k/v must be [ntok, Hkv, D] with one slot per token")
+    on_device(plan.device_index, v=v, kv_pool=kv_pool, slot_mapping=slot_mapping, out=out)
     if kv_pool.dtype is torch.uint8:
         q_out, k_out = rotary(q, k, positions, plan, q_weight=q_weight, k_weight=k_weight, eps=eps)
         paged.kv_append(k_out, v.contiguous(), kv_pool, slot_mapping)

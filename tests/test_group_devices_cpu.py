@@ -61,3 +61,66 @@ def test_rotary_takes_subclasses_of_tensor(launched):
     with pytest.raises(TypeError):
         rotary.rotary(on(torch.zeros((4, 2, 64))), _bf(4, 1, 64), pos, plan)
     assert launched == ["_append"]
+
+
+def _each_on_another(call, operands, launched):
+    """call(**operands) launches; with any one operand on GPU 1 it raises and does not."""
+    call(**operands)
+    assert len(launched) == 1
+    for name in operands:
+        moved = dict(operands)
+        t = moved[name]
+        moved[name] = [on(t[0].clone(), 1)] if isinstance(t, list) else on(t.clone(), 1)
+        with pytest.raises(ValueError, match="is on|are on"):
+            call(**moved)
+        assert len(launched) == 1, name
+
+
+@pytest.mark.parametrize("append", [False, True])
+def test_rotary(launched, append):
+    plan = _plan(rotary.RotaryPlan, 64)
+    operands = dict(q=_bf(4, 2, 64), k=_bf(4, 1, 64),
+                    positions=on(torch.zeros((1, 4), dtype=torch.int32)),
+                    q_weight=_bf(64), k_weight=_bf(64))
+    if not append:
+        _each_on_another(lambda **kw: rotary.rotary(plan=plan, **kw), operands, launched)
+        return
+    operands.update(v=_bf(4, 1, 64), kv_pool=_bf(2, 1, 2, 16, 64),
+                    slot_mapping=on(torch.zeros(4, dtype=torch.int64)), out=_bf(4, 2, 64))
+    _each_on_another(lambda **kw: rotary.rotary_append(plan=plan, **kw), operands, launched)
+
+
+def test_beam_select(launched, monkeypatch):
+    monkeypatch.setattr(beam, "_workspace", lambda *a: 256)
+    operands = dict(logits=_bf(2, 3, 50), scores=on(torch.zeros((2, 3))),
+                    finished=on(torch.zeros((2, 3), dtype=torch.bool)))
+    _each_on_another(lambda **kw: beam.beam_select(n=4, **kw), operands, launched)
+
+
+def test_reorder_rows(launched):
+    ids = torch.zeros((1, 3), dtype=torch.int32)
+    operands = dict(pools=[_bf(1, 4, 8)], slots=on(ids), parents=on(ids.clone()))
+    _each_on_another(lambda **kw: beam.reorder_rows(**kw), operands, launched)
+
+
+@pytest.mark.parametrize("rows", [[0, 1], [0]])
+def test_shared_prefix_attention(launched, monkeypatch, rows):
+    monkeypatch.setattr(paged._capi, "call", lambda *a: launched.append(a[0]))
+    monkeypatch.setattr(paged, "sm_count", lambda d: 148)
+    groups = _plan(paged.PrefixGroups, [(rows, 32)], 2, 4, 2, 64, sms=148)
+    assert groups.ntiles == (len(rows) > 1)
+    operands = dict(q=_bf(2, 4, 64), kv_pool=_bf(8, 2, 2, 16, 64),
+                    block_table=on(torch.zeros((2, 4), dtype=torch.int32)),
+                    ctx_len=on(torch.zeros(2, dtype=torch.int32)), out=_bf(2, 4, 64),
+                    lse_out=on(torch.zeros(8)))
+    ws = paged.SharedPrefixWorkspace("cpu")
+    ws.device_index = 0
+    call = lambda **kw: paged.shared_prefix_attention(scale=0.1, groups=groups, workspace=ws,  # noqa: E731
+                                                      **kw)
+    _each_on_another(call, operands, launched)
+    other = paged.SharedPrefixWorkspace("cpu")
+    other.device_index = 1
+    if groups.ntiles:
+        with pytest.raises(ValueError):
+            paged.shared_prefix_attention(scale=0.1, groups=groups, workspace=other, **operands)
+        assert len(launched) == 1
