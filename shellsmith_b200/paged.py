@@ -513,24 +513,40 @@ def tail_split_plan(batch: int, q_heads: int, kv_heads: int, max_pages: int,
 
 
 class SharedPrefixWorkspace:
-    """Reusable scratch of shared_prefix_attention (the parts); grows when needed."""
+    """Reusable scratch of shared_prefix_attention (the parts); grows when needed.
+
+    Memory that queued work may still use is not given back: a stream other than the one
+    the buffer came from is recorded with the allocator, and a buffer that a CUDA graph
+    captured is kept with the workspace (which has to live as long as the graph).
+    """
 
     def __init__(self, device: str | torch.device = "cuda"):
         self.device = torch.device(device)
         self._buffer = torch.empty(0, dtype=torch.float32, device=device)
         self.device_index = self._buffer.get_device()
         self._floats = 0
+        self._home = 0          # the stream that the buffer was allocated on
+        self._captured = False  # a graph holds the buffer's address
+        self._kept: list = []   # outgrown buffers that one does
 
     def parts(self, rows: int, dim: int, prefix_splits: int, splits: int) -> tuple:
         """Addresses of prefix_out, prefix_lse, part_out, part_lse for `rows` (row, head)s,
-        and of the work counters."""
+        and of the work counters, for a call on the current stream."""
         pre, own = rows * prefix_splits, rows * splits
         at1 = pre * dim                          # D is a multiple of 64: aligned steps
         at2 = at1 + own * dim
         need = at2 + pre + own + rows // 1024 + 1
+        stream = stream_of(self._buffer)
         if self._floats < need:
+            if self._captured:
+                self._kept.append(self._buffer)
+                self._captured = False
             self._buffer = torch.empty(need, dtype=torch.float32, device=self.device)
-            self._floats = need
+            self._floats, self._home = need, stream
+        elif stream != self._home:
+            self._buffer.record_stream(torch.cuda.current_stream(self.device_index))
+        if stream and torch.cuda.is_current_stream_capturing():  # never the default one
+            self._captured = True
         base = self._buffer.data_ptr()
         return (base, base + 4 * at2, base + 4 * at1, base + 4 * (at2 + pre),
                 base + 4 * (at2 + pre + own))

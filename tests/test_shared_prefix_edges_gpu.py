@@ -2,8 +2,12 @@
 over many units of work, infinities in the cache, long sequences without a group. Cases, the
 64-bit reference and the bars are those of the operator's own tests."""
 
+import numpy as np
 import pytest
-from test_shared_prefix_gpu import _case, _check
+import torch
+from test_shared_prefix_gpu import _case, _check, _expect
+
+from shellsmith_b200 import _capi, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -18,3 +22,95 @@ def test_many_short_tails(cuda, hq, hkv, D, longest):
     case = _case(cuda, groups, tails, hq, hkv, D, seed=longest)
     for _ in range(3):
         _check(cuda, case)
+
+
+def _prepared(cuda, case, ws, scale=0.0625):
+    """The call of a case with everything on the device before it: nothing in it waits."""
+    q, pool, table, ctx, plan = case
+    groups = paged.PrefixGroups(plan, q.shape[0], q.shape[1], pool.shape[1], q.shape[2], device=cuda)
+    t, c = torch.from_numpy(table).to(cuda), torch.from_numpy(ctx.astype(np.int32)).to(cuda)
+    return lambda: paged.shared_prefix_attention(q, pool, t, c, scale, groups, workspace=ws)
+
+
+def _matches(out, case, scale=0.0625):
+    q, pool, table, ctx, _ = case
+    want, _, mass = _expect(q, pool, table, ctx, scale)
+    tol = (2.0 ** -8 + 3e-4) * mass + 2.0 ** -8 * 1.01 * np.abs(want) + 1e-6
+    got = out.double().cpu().numpy()
+    assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all()
+
+
+def test_workspace_memory_outlives_the_work_on_it(cuda):
+    """A workspace from one stream grows on another: its old memory is not handed out on the
+    first while the second still has work on it."""
+    small = _case(cuda, [(3, 160)], [1, 9, 30], 16, 2, 256, seed=1)
+    large = _case(cuda, [(9, 1600)], [1 + 31 * i for i in range(9)], 16, 2, 256, seed=2)
+    ws = paged.SharedPrefixWorkspace(cuda)
+    one, two = _prepared(cuda, small, ws), _prepared(cuda, large, ws)
+    one()
+    floats, old = ws._floats, ws._buffer.data_ptr()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)   # about 0.1 s: the call below is still queued
+        a = one()
+        b = two()
+    assert ws._floats > floats
+    fresh = torch.empty(floats, dtype=torch.float32, device=cuda)
+    assert fresh.data_ptr() != old
+    assert not side.query()              # it was still queued
+    fresh.fill_(float("nan"))
+    torch.cuda.synchronize()
+    _matches(a, small)
+    _matches(b, large)
+
+
+def test_workspace_of_a_captured_call(cuda):
+    """A graph keeps the memory that it was captured with when the workspace grows."""
+    small = _case(cuda, [(3, 160)], [1, 9, 30], 16, 2, 256, seed=1)
+    large = _case(cuda, [(9, 1600)], [1 + 31 * i for i in range(9)], 16, 2, 256, seed=2)
+    ws = paged.SharedPrefixWorkspace(cuda)
+    one, two = _prepared(cuda, small, ws), _prepared(cuda, large, ws)
+    one()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = one()
+    floats, old = ws._floats, ws._buffer.data_ptr()
+    b = two()
+    torch.cuda.synchronize()
+    taken = [torch.zeros(floats, device=cuda) for _ in range(4)]
+    assert old not in [t.data_ptr() for t in taken]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not any(t.any() for t in taken)
+    _matches(out, small)
+    _matches(b, large)
+
+
+def test_calls_back_to_back_on_one_workspace(cuda):
+    """Calls of different shapes, contexts and counters queued on a side stream with nothing
+    between them: each one's first kernel starts while the last of the one before ends, on
+    the same parts."""
+    cases = [_case(cuda, [(8, 1600)], [1 + 9 * i for i in range(8)], 16, 2, 256, seed=9),
+             _case(cuda, [(5, 48), (40, 320)], [1 + (7 * i) % 90 for i in range(45)], 24, 8, 128, seed=3),
+             _case(cuda, [(3, 5000)], [2000, 1, 40], 8, 8, 64, seed=4),
+             _case(cuda, [(2, 160)], [-100, None], 16, 2, 256, seed=5)]
+    ws = paged.SharedPrefixWorkspace(cuda)
+    calls = [_prepared(cuda, c, ws) for c in cases]
+    for call in calls:  # grown to its size, kernels loaded
+        call()
+    torch.cuda.synchronize()
+    order = [0, 1, 2, 3, 3, 2, 0, 0, 1, 3, 1, 2, 0, 3, 2, 1] * 4
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # the queue fills before the first one runs
+        outs = [calls[i]() for i in order]
+    side.synchronize()
+    _capi.check_device(side.cuda_stream)
+    first = {}
+    for i, out in zip(order, outs):
+        if i not in first:
+            first[i] = out
+            _matches(out, cases[i])
+        assert torch.equal(out, first[i])
