@@ -164,6 +164,21 @@ __device__ __forceinline__ void mma_elected(uint32_t elected, uint32_t d_tmem, u
       : "memory");
 }
 
+// The same, but the rows (TMEM lanes) whose bits are set in `off` keep what D held.
+__device__ __forceinline__ void mma_elected_rows(uint32_t elected, uint32_t d_tmem,
+                                                 uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                                 const uint32_t (&off)[4], bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%6, %7, %8, %9}, p;\n\t}"
+      :
+      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u),
+        "r"(elected), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+      : "memory");
+}
+
 // Barrier of the softmax warps that ORs a predicate over them.
 __device__ __forceinline__ bool soft_any(bool pred) {
   int r;
@@ -361,9 +376,19 @@ __global__ void __maxnreg__(112)
       }
       __syncwarp();
     };
+    // A row's O takes the pages that the row attends to and no others: a page past its context
+    // may hold an Inf or NaN that another member wrote, and 0 * Inf would be in its sum. Lane
+    // j: the page of this split at which rows j, j + 32, j + 64 and j + 96 end.
+    int end[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int row = row_of(lane + 32 * x);
+      end[x] = row < 0 ? npages : min(pages_of(row / a.Hq) - p0, npages);
+    }
     wait(qfull, 0);
     tc::fence_after();
     scores(0);
+    const bool uneven = __any_sync(0xffffffffu, min(min(end[0], end[1]), min(end[2], end[3])) < npages);
     for (int i = 0; i < ntiles; ++i) {
       if (i + 1 < ntiles) scores(i + 1);
       const int st = i % S::STAGES;
@@ -372,10 +397,24 @@ __global__ void __maxnreg__(112)
       tc::fence_after();
       __syncwarp();
       const uint32_t vb = smem_addr(sm + (S::STAGES + st) * S::TILE_BYTES);
+      const uint32_t pb = tmem + S::T_S + (i & 1) * S::TOK;
+      const int page0 = i * S::PAGES, pages = npages - page0;
+      if (!uneven && pages >= S::PAGES) {
 #pragma unroll
-      for (int kk = 0; kk < S::PAGES; ++kk)
-        mma_elected(one, tmem, tmem + S::T_S + (i & 1) * S::TOK + 8 * kk,
-                    tc::smem_desc(vb + kk * S::PAGE_BYTES, 2048, 1024), kIdO, i > 0 || kk > 0);
+        for (int kk = 0; kk < S::PAGES; ++kk)
+          mma_elected(one, tmem, pb + 8 * kk, tc::smem_desc(vb + kk * S::PAGE_BYTES, 2048, 1024),
+                      kIdO, i > 0 || kk > 0);
+      } else {  // a product is a page: of the last tile those that are there
+#pragma unroll 1
+        for (int kk = 0; kk < min(S::PAGES, pages); ++kk) {
+          uint32_t off[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) off[x] = __ballot_sync(0xffffffffu, end[x] <= page0 + kk);
+          mma_elected_rows(one, tmem, pb + 8 * kk,
+                           tc::smem_desc(vb + kk * S::PAGE_BYTES, 2048, 1024), kIdO, off,
+                           i > 0 || kk > 0);
+        }
+      }
       if (one) {
         tc::commit(&ofull[i & 1]);
         tc::commit(&vfree[st]);

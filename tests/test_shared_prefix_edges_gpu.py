@@ -114,3 +114,55 @@ def test_calls_back_to_back_on_one_workspace(cuda):
             first[i] = out
             _matches(out, cases[i])
         assert torch.equal(out, first[i])
+
+
+def _decode(cuda, case, scale, sms=None):
+    q, pool, table, ctx, plan = case
+    groups = paged.PrefixGroups(plan, q.shape[0], q.shape[1], pool.shape[1], q.shape[2], device=cuda,
+                                sms=sms)
+    t, c = torch.from_numpy(table).to(cuda), torch.from_numpy(ctx.astype(np.int32)).to(cuda)
+    out = paged.shared_prefix_attention(q, pool, t, c, scale, groups)
+    _capi.check_device()
+    return out, paged.paged_decode_attention(q, pool, t, c, scale)
+
+
+@pytest.mark.parametrize("hq,hkv,D", [(16, 2, 256), (24, 8, 128), (8, 8, 64), (64, 1, 64)])
+@pytest.mark.parametrize("sms", [1, 148])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_pages_past_a_members_context_do_not_reach_it(cuda, hq, hkv, D, sms, value):
+    """Members whose contexts end inside the shared pages, which hold infinities or NaN past
+    them, as K or as V: their rows are those of the finite tokens that they attend to."""
+    pages = 40
+    tails = [5, -1, -16, -100, -300, None, 0, -17, -639 + 16]
+    case = _case(cuda, [(len(tails), pages * 16)], tails, hq, hkv, D, seed=7)
+    q, pool, table, ctx, _ = case
+    shared = torch.from_numpy(table[0, :pages].astype(np.int64)).to(cuda)
+    for last, which in ((20, 1), (1, 1), (39, 1), (30, 0), (7, 0)):
+        bad = pool.clone()
+        bad[shared[last:], :, which] = value
+        rows = [i for i, n in enumerate(ctx) if n <= 16 * last]
+        assert rows and len(rows) < len(tails)
+        now = (q, bad, table, ctx, case[4])
+        out, plain = _decode(cuda, now, 0.06, sms)
+        want, _, mass = _expect(q, pool, table, ctx, 0.06)
+        tol = (2.0 ** -8 + 3e-4) * mass + 2.0 ** -8 * 1.01 * np.abs(want) + 1e-6
+        got = out.double().cpu().numpy()
+        assert np.isfinite(got[rows]).all() and torch.isfinite(plain[rows]).all()
+        assert (np.abs(got - want)[rows] <= tol[rows]).all()
+
+
+@pytest.mark.parametrize("pages", [37, 38, 39, 40])
+@pytest.mark.parametrize("D", [64, 256])
+def test_an_infinite_value_stays_infinite(cuda, pages, D):
+    """V of +Inf in one column of the last shared page, inside a tile of the kernel or not:
+    that column is +Inf, as p > 0 there, and the others are what they were."""
+    case = _case(cuda, [(3, pages * 16)], [1, 30, 17], 8, 2, D, seed=8)
+    q, pool, table, ctx, _ = case
+    want, plain = _decode(cuda, case, 0.05)
+    bad = pool.clone()
+    token, col = 5, 24                                     # stored at chunk 3 ^ 5 of the row
+    bad[int(table[0, pages - 1]), :, 1, token, ((col // 8) ^ token) * 8 + col % 8] = float("inf")
+    out, plain = _decode(cuda, (q, bad, table, ctx, case[4]), 0.05)
+    assert torch.isposinf(out[..., col]).all() and torch.isposinf(plain[..., col]).all()
+    rest = torch.arange(D, device=cuda) != col
+    assert torch.equal(out[..., rest], want[..., rest])
