@@ -808,11 +808,12 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
         t0 = fmaxf(t0, __shfl_xor_sync(kAll, t0, off));
         t1 = fmaxf(t1, __shfl_xor_sync(kAll, t1, off));
       }
-      // The first token of every page counts, so t0 / t1 are finite for finite scores.
+      // The maxima are -inf while every score is (a key of -Inf): each p is 0 then.
       const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-      const float c0 = exp2f(m0 - n0), c1 = exp2f(m1 - n1);
-      const float p0 = exp2f(x0 - n0), p1 = exp2f(x1 - n1);
-      const float p2 = exp2f(x2 - n0), p3 = exp2f(x3 - n1);
+      const float r0 = n0 == -CUDART_INF_F ? 0.f : n0, r1 = n1 == -CUDART_INF_F ? 0.f : n1;
+      const float c0 = exp2f(m0 - r0), c1 = exp2f(m1 - r1);
+      const float p0 = exp2f(x0 - r0), p1 = exp2f(x1 - r1);
+      const float p2 = exp2f(x2 - r0), p3 = exp2f(x3 - r1);
       l0 = fmaf(l0, c0, p0 + p2);
       l1 = fmaf(l1, c1, p1 + p3);
       m0 = n0;
@@ -846,7 +847,7 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
     }
     // O^T: this lane holds dims d0 + 16 mt (+ 8) of heads h0, h0 + 1.
     const int d0 = lane >> 2, h0 = 2 * (lane & 3);
-    const float i0 = 1.f / l0, i1 = 1.f / l1;
+    const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
     const size_t part = ((size_t)cur.b * a.Hq + cur.head0 + h0) * a.num_splits + cur.split;
     float* w0 = a.part_out + part * D + d0;
     float* w1 = w0 + (size_t)a.num_splits * D;

@@ -166,3 +166,24 @@ def test_an_infinite_value_stays_infinite(cuda, pages, D):
     assert torch.isposinf(out[..., col]).all() and torch.isposinf(plain[..., col]).all()
     rest = torch.arange(D, device=cuda) != col
     assert torch.equal(out[..., rest], want[..., rest])
+
+
+@pytest.mark.parametrize("hq,hkv,D", [(16, 2, 256), (12, 1, 128), (8, 8, 64)])
+def test_tokens_with_scores_of_minus_infinity_weigh_nothing(cuda, hq, hkv, D):
+    """Keys of -Inf against a positive entry of q: whole pages of them, first in the prefix,
+    first in a sequence's own pages (and in a unit of those by themselves), and single ones."""
+    case = _case(cuda, [(3, 320)], [200, 17, 90], hq, hkv, D, seed=11, single=[60])
+    q, pool, table, ctx, _ = case
+    q[..., 0] = q[..., 0].abs() + 1
+    def kill(b, tokens):
+        for t in tokens:
+            page, row = int(table[b, t // 16]), t % 16
+            pool[page, :, 0, row, 8 * (row & 7)] = -float("inf")  # column 0 of its row
+    kill(0, range(0, 33))                # two pages of the prefix and a token
+    kill(0, range(320, 320 + 64))        # the first unit of row 0's own pages
+    kill(1, range(320, 336))             # its first own page, one token left
+    kill(2, [320, 350, 409])
+    kill(3, range(0, 16))
+    _check(cuda, case)
+    for splits in (1, 2, 8):
+        _check(cuda, case, pages_per_split=splits)
