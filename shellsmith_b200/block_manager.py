@@ -187,6 +187,12 @@ class BlockManager:
         self.dirty_rows.add(slot)
         return slot
 
+    def freed_by(self, slots) -> int:
+        """Pages that nobody else owns: what these sequences would give back together."""
+        pages = [p for s in slots for p in self.pages[s]]
+        owned, count = np.unique(np.asarray(pages, np.int64), return_counts=True)
+        return int((self.refcount[owned] == count).sum())
+
     def replace(self, slot: int, pages: list, tokens: int) -> None:
         """Give an active slot other pages, which the caller owns already (a beam that
         continues another one); its old pages lose an owner."""

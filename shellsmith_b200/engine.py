@@ -215,6 +215,10 @@ class HybridCacheEngine:
                 owned.append(pages[full])
         return owned
 
+    @property
+    def free_snapshot_rows(self) -> int:
+        return len(self._free_snapshot_rows)
+
     def snapshot(self, slot: int) -> "PagedSnapshot":
         """An immutable copy of a live sequence's cache: full pages shared, the partial
         last page (which the sequence keeps writing) and the GDN state copied."""
@@ -250,13 +254,16 @@ class HybridCacheEngine:
         self._free_snapshot_rows.append(snap.row)
         snap.row = None
 
-    def reorder(self, slots, parents) -> list:
+    def reorder(self, slots, parents, reuse_pages: bool = False) -> list:
         """Let the sequences in `slots` follow their beams: the j-th continues what
         slots[parents[j]] holds. Returns the new slots.
 
         The first child of a beam keeps its slot; each later one takes the slot of a beam
         without children (beam.reorder_rows' rule): its GDN state and tap rows are copied
         there on the device, full pages are shared and the partial last page is copied.
+        Raises MemoryError, with nothing changed, where the free pages do not hold the
+        copied ones; with reuse_pages those count too that the beams without children
+        give back (of beams of one length always enough).
         """
         slots, parents = [int(s) for s in slots], [int(p) for p in parents]
         if len(parents) != len(slots) or any(p < 0 or p >= len(slots) for p in parents):
@@ -268,23 +275,30 @@ class HybridCacheEngine:
             return new.tolist()
         P, blocks = self.cfg.page_size, self.blocks
         partial = sum(int(blocks.lengths[s]) % P != 0 for s, _ in copies)
-        if partial > blocks.free_pages:  # before anything changes
-            raise MemoryError(f"{partial} pages needed, {blocks.free_pages} free")
+        room = blocks.free_pages
+        if reuse_pages:
+            room += blocks.freed_by([to for _, to in copies])
+        if partial > room:  # before anything changes
+            raise MemoryError(f"{partial} pages needed, {room} free")
         tables = torch.tensor([slots, parents], dtype=torch.int32, device=self.device)
         pools = [self.state] if self.taps is None else [self.state, self.taps]
         beam.reorder_rows(pools, tables[:1], tables[1:])
-        src, dst = [], []
+        # Every slot's old pages go before the first new one is taken; no source is among
+        # the slots that lose theirs.
+        moves = []
         for source, to in copies:
             tokens = int(blocks.lengths[source])
-            pages = blocks.pages[source][:blocks.pages_for(tokens)]
-            owned = pages[:tokens // P]
-            blocks.share(owned)
+            pages = blocks.pages[source]
+            blocks.share(pages[:tokens // P])
+            moves.append((to, tokens, pages[:tokens // P], pages[tokens // P:tokens // P + 1]))
+        for to, tokens, full, _ in moves:
+            blocks.replace(to, full, tokens // P * P)
+        src, dst = [], []
+        for to, tokens, _, last in moves:
             if tokens % P:
-                fresh = blocks.take_pages(1)
-                src.append(pages[tokens // P])
-                dst += fresh
-                owned = owned + fresh
-            blocks.replace(to, owned, tokens)
+                blocks.extend(to, tokens)
+                src += last
+                dst.append(blocks.pages[to][-1])
         self._copy_pages(src, dst)
         return new.tolist()
 

@@ -151,7 +151,7 @@ class BeamSearch:
             old = self.beams[p]
             chosen.append(Beam(old.tokens if old.finished else old.tokens + [t], s,
                                old.finished or t == self.stop))
-        self.slots = self.cache.reorder(self.slots, parents)
+        self.slots = self.cache.reorder(self.slots, parents, reuse_pages=True)
         self.beams = chosen
 
     def search(self, prompt: list, beams: int, max_tokens: int) -> list:

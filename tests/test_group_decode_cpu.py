@@ -151,3 +151,13 @@ def test_group_fake_kernels_propagate_shapes():
         assert (best.dtype, parents.dtype, tokens.dtype) == (f32, i32, i32)
         slots = make(3, 4, dtype=i32)
         assert ops.reorder_rows([make(2, 12, 64)], slots, slots).shape == slots.shape
+
+
+def test_freed_by_counts_pages_that_nobody_else_owns():
+    blocks = BlockManager(num_pages=32, max_seqs=6, page_size=16, max_pages_per_seq=8)
+    a, b = blocks.admit("a", 40), blocks.admit("b", 20)
+    shared = blocks.pages[a][:2]
+    blocks.share(shared)
+    c = blocks.adopt("c", shared + blocks.take_pages(1), 40)
+    for slots, pages in (([a], 1), ([b], 2), ([c], 1), ([a, c], 4), ([a, b, c], 6), ([], 0)):
+        assert blocks.freed_by(slots) == pages
