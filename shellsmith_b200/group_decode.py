@@ -58,19 +58,27 @@ class BeamSearch:
         if eng.blocks.free_slots < beams or eng.blocks.free_pages < pages:
             raise MemoryError(f"{beams} slots and {pages} pages needed, "
                               f"{eng.blocks.free_slots} and {eng.blocks.free_pages} free")
-        slot = eng.admit("beam", len(prompt))
-        self.slots = [slot]
-        self._logits = self._prefill(slot, prompt)
-        if beams > 1:
-            snap = eng.snapshot(slot)
-            self.slots += [eng.fork(snap, owner="beam") for _ in range(beams - 1)]
-            eng.drop_snapshot(snap)
-        self.beams = [Beam() for _ in range(beams)]
-        # Until the beams differ only the first one counts.
-        self._scores = torch.full((1, beams), -float("inf"), device=eng.device)
-        self._scores[0, 0] = 0.0
-        self._logits = self._logits.expand(beams, -1)
-        self._choose()
+        if beams > 1 and not eng.free_snapshot_rows:
+            raise MemoryError("a snapshot row is needed to fork the beams, none is free")
+        self.slots = [eng.admit("beam", len(prompt))]
+        try:
+            self._logits = self._prefill(self.slots[0], prompt)
+            if beams > 1:
+                snap = eng.snapshot(self.slots[0])
+                try:
+                    for _ in range(beams - 1):
+                        self.slots.append(eng.fork(snap, owner="beam"))
+                finally:
+                    eng.drop_snapshot(snap)
+            self.beams = [Beam() for _ in range(beams)]
+            # Until the beams differ only the first one counts.
+            self._scores = torch.full((1, beams), -float("inf"), device=eng.device)
+            self._scores[0, 0] = 0.0
+            self._logits = self._logits.expand(beams, -1)
+            self._choose()
+        except BaseException:
+            self.close()
+            raise
 
     def _prefill(self, slot: int, ids: list) -> torch.Tensor:
         eng, model, c, dev = self.cache, self.model, self.cache.cfg, self.cache.device
@@ -103,7 +111,11 @@ class BeamSearch:
 
     # ---------------------------------------------------------------- steps
     def step(self) -> bool:
-        """One token for every beam, then the best beams go on; False when all are done."""
+        """One token for every beam, then the best beams go on; False when all are done.
+
+        Raises OutOfPages, with nothing changed, where the pool cannot hold the token: the
+        step may be taken again when there is room.
+        """
         if all(b.finished for b in self.beams):
             return False
         eng, model, c = self.cache, self.model, self.cache.cfg
@@ -142,17 +154,17 @@ class BeamSearch:
         count = len(self.beams)
         done = torch.tensor([[b.finished for b in self.beams]], device=self.cache.device)
         pad = 0 if self.stop is None else self.stop
-        self._scores, parents, tokens = beam.beam_select(
-            self._logits[None].contiguous(), self._scores, count, finished=done, pad_token=pad)
+        best, parents, tokens = beam.beam_select(self._logits[None].contiguous(), self._scores,
+                                                 count, finished=done, pad_token=pad)
         parents, tokens = parents[0].tolist(), tokens[0].tolist()
-        scores = self._scores[0].tolist()
+        scores = best[0].tolist()
         chosen = []
         for p, t, s in zip(parents, tokens, scores):
             old = self.beams[p]
             chosen.append(Beam(old.tokens if old.finished else old.tokens + [t], s,
                                old.finished or t == self.stop))
         self.slots = self.cache.reorder(self.slots, parents, reuse_pages=True)
-        self.beams = chosen
+        self.beams, self._scores = chosen, best
 
     def search(self, prompt: list, beams: int, max_tokens: int) -> list:
         """The best continuations of the prompt, up to max_tokens long, best first."""

@@ -64,6 +64,36 @@ def test_a_search_goes_on_when_there_is_room_again(cuda):
     assert found[0][0] == found[1][0] and torch.equal(found[0][1], found[1][1])
 
 
+def test_start_without_a_snapshot_row_opens_nothing(cuda):
+    cfg = _cfg(snapshot_rows=1)
+    model = ToyHybridModel(cfg, device=cuda)
+    eng, search = _search(cuda, cfg, model)
+    other = eng.admit("other", 10)
+    snap = eng.snapshot(other)
+    free = eng.blocks.free_pages
+    with pytest.raises(MemoryError):
+        search.start([1, 2, 3], 2)
+    assert not search.slots and eng.blocks.free_pages == free
+    search.start([1, 2, 3], 1)            # one beam needs none
+    search.close()
+    eng.drop_snapshot(snap)
+    search.start([1, 2, 3], 2)
+    search.close()
+    assert eng.blocks.free_pages == free + 1
+
+
+def test_an_error_in_start_opens_nothing(cuda, monkeypatch):
+    cfg = _cfg()
+    model = ToyHybridModel(cfg, device=cuda)
+    eng, search = _search(cuda, cfg, model)
+    monkeypatch.setattr(eng, "reorder", lambda *a, **kw: 1 / 0)
+    free, rows = eng.blocks.free_pages, eng.free_snapshot_rows
+    with pytest.raises(ZeroDivisionError):
+        search.start([1, 2, 3], 3)
+    assert not search.slots and not search.beams
+    assert eng.blocks.free_pages == free and eng.free_snapshot_rows == rows
+
+
 def test_reorder_takes_the_pages_that_its_beams_give_back(cuda):
     eng = HybridCacheEngine(_cfg(num_pages=8), device=cuda)
     slots = [eng.admit(i, 20) for i in range(4)]
