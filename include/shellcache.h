@@ -523,7 +523,7 @@ int sc_rotary_append(const sc_bf16* q, const sc_bf16* k, const sc_bf16* v,
  *               whose block table lists those pages
  * members       rows of the batch, each with prefix_pages > 0 in exactly one tile
  * prefix_pages_per_split, prefix_splits  the split of the shared pages
- * pages_per_split (at most 32), num_splits  the split of each sequence's other pages
+ * pages_per_split, num_splits  the split of each sequence's other pages
  * prefix_out [B, Hq, prefix_splits, D], prefix_lse [B, Hq, prefix_splits], part_out
  * [B, Hq, num_splits, D], part_lse [B, Hq, num_splits]: fp32 scratch
  * counters      ceil(B / 1024) int32 of scratch

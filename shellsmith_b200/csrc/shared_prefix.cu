@@ -593,7 +593,6 @@ __global__ void __maxnreg__(112)
 constexpr int kTailWarps = 2;
 constexpr int kTailStages = 3;
 constexpr int kTailHeads = 8;        // query heads of a unit
-constexpr int kTailMaxPages = 32;    // pages of a unit: a lane holds the id of one
 constexpr int kSlabRows = 1024;      // rows whose units one counter hands out
 
 struct TailArgs {
@@ -621,7 +620,9 @@ __device__ __forceinline__ OwnPages own_pages(int ctx, int first_page, int max_p
   return o;
 }
 
-template <int D>
+// kLong: units of more than 32 pages, whose ids the warp's lanes read 32 at a time. With that in
+// every launch 128 sequences on 8,208 tokens took 48.9 us, without 47.8.
+template <int D, bool kLong>
 __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
   constexpr int ROW = D * 2, KV = kPageTok * ROW, STAGE = 2 * KV, KSTEPS = D / 16;
   constexpr unsigned kAll = 0xffffffffu;
@@ -672,7 +673,8 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
 
   struct Unit {
     int b, kvh, head0, heads, split, n, tokens;  // n pages; tokens of them count
-    int page;                                    // lane i: the id of page i
+    int first;                                   // (kLong) the first one's place in the table
+    int page;                                    // lane i: the id of page i of 32
   };
   // Unit t of the slab: chunk t / groups of the rows' chunks laid end to end. Uniform over
   // the warp; u.n == 0 past the last one.
@@ -702,6 +704,7 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
     u.split = chunk;
     u.n = min(a.pages_per_split, pages - p0);
     u.tokens = min(u.n * kPageTok, tokens - p0 * kPageTok);
+    if constexpr (kLong) u.first = skip + p0;
     u.page = lane < u.n ? a.block_table[(size_t)u.b * a.max_pages + skip + p0 + lane] : 0;
     u.kvh = hg / a.HG;
     u.head0 = u.kvh * a.G + (hg - u.kvh * a.HG) * kTailHeads;
@@ -711,8 +714,12 @@ __global__ void __maxnreg__(168) tail_kernel(const TailArgs a) {
 
   const uint64_t once = read_once();
   int issued = 0, consumed = 0;  // pages of all units, in order through the stages
-  const auto issue = [&](const Unit& u, int i) {
-    int page = __shfl_sync(kAll, u.page, i);
+  const auto issue = [&](Unit& u, int i) {
+    if constexpr (kLong)
+      if (i > 0 && (i & 31) == 0)
+        u.page = i + lane < u.n
+                     ? a.block_table[(size_t)u.b * a.max_pages + u.first + i + lane] : 0;
+    int page = __shfl_sync(kAll, u.page, kLong ? i & 31 : i);
     if (lane == 0) {
       if (page < 0 || page >= a.num_pages) {
         flag_device(a.status, DEV_BAD_INDEX);
@@ -1064,12 +1071,14 @@ int launch_shared(const CUtensorMap* maps, const PrefixArgs& p, const MergeArgs&
     if (err == cudaSuccess)
       err = cudaFuncSetAttribute(prefix_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                  cudaSharedmemCarveoutMaxShared);
-    if (err == cudaSuccess)
-      err = cudaFuncSetAttribute(tail_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)tail_smem);
-    if (err == cudaSuccess)
-      err = cudaFuncSetAttribute(tail_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                 cudaSharedmemCarveoutMaxShared);
+    for (auto tail : {tail_kernel<D, false>, tail_kernel<D, true>}) {
+      if (err == cudaSuccess)
+        err = cudaFuncSetAttribute(tail, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)tail_smem);
+      if (err == cudaSuccess)
+        err = cudaFuncSetAttribute(tail, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                   cudaSharedmemCarveoutMaxShared);
+    }
     if (err != cudaSuccess)
       return set_error(SC_ERR_CUDA, "%s: smem attribute: %s", name, cudaGetErrorString(err));
     configured[dev] = 1;
@@ -1081,7 +1090,8 @@ int launch_shared(const CUtensorMap* maps, const PrefixArgs& p, const MergeArgs&
   // Two CTAs an SM (one while a prefix CTA is there), fewer where there is less work.
   const long long units = (long long)std::min(p.B, kSlabRows) * t.Hkv * t.HG * t.num_splits;
   const int ctas = (int)std::min(2ll * 148, (units + kTailWarps - 1) / kTailWarps);
-  err = launch_pdl(tail_kernel<D>, dim3(ctas, p.slabs), dim3(kTailWarps * 32), tail_smem, s, t);
+  err = launch_pdl(t.pages_per_split > 32 ? tail_kernel<D, true> : tail_kernel<D, false>,
+                   dim3(ctas, p.slabs), dim3(kTailWarps * 32), tail_smem, s, t);
   if (err != cudaSuccess)
     return set_error(SC_ERR_CUDA, "%s: launch: %s", name, cudaGetErrorString(err));
   // As many warps a row (a power of two, at most 8) as the GPU holds at once. 128 rows of 8
@@ -1131,8 +1141,6 @@ extern "C" int sc_shared_prefix_attention(
   SC_REQUIRE(B <= 65535 && ntiles <= 65535 && Hkv <= 65535 && Hkv * ((Hq / Hkv + 7) / 8) <= 65535 &&
                  num_pages * Hkv * 2 < (1ll << 31),
              SC_ERR_INVALID, "%s: grid or pool too large", name);
-  SC_REQUIRE(pages_per_split <= sc::kTailMaxPages, SC_ERR_UNSUPPORTED,
-             "%s: %d pages per split, at most %d", name, pages_per_split, sc::kTailMaxPages);
   const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   SC_REQUIRE(aligned(q) && aligned(kv_pool) && aligned(out) && aligned(prefix_out) &&
                  aligned(part_out) && aligned(tiles),

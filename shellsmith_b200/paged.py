@@ -497,17 +497,24 @@ def prefix_split_plan(tile_pages: list, kv_heads: int, head_dim: int, sms: int,
     return pps, max(1, -(-longest // pps))
 
 
+MOST_PARTS = 1024  # parts of one (row, head) that the merge takes
+
+
 def tail_split_plan(batch: int, q_heads: int, kv_heads: int, max_pages: int,
-                    pages_per_split: int | None, total_pages: int | None, sms: int) -> tuple:
+                    pages_per_split: int | None, total_pages: int | None, sms: int,
+                    most_splits: int | None = None) -> tuple:
     """(pages_per_split, num_splits) of the sequences' own pages beside a prefix: units of
     work of up to 16 pages, small enough that every warp of two CTAs an SM gets some. 64
     sequences of U[1, 2048] tokens took 35.5 / 32.1 / 31.2 / 36.3 us in units of 4 / 8 / 16 /
-    32 pages, 15 of U[1, 777] 13.5 / 13.4 / 17.3 / 26.8."""
+    32 pages, 15 of U[1, 777] 13.5 / 13.4 / 17.3 / 26.8. Units double on where the longest
+    sequence would have more than most_splits of them (a limit, not a matter of speed)."""
     if not pages_per_split:
         groups = kv_heads * ((q_heads // kv_heads + 7) // 8)
         work = (total_pages or batch * max_pages) * groups
         pages_per_split = 4
         while pages_per_split < 16 and work / (2 * pages_per_split) >= 4 * sms:
+            pages_per_split *= 2
+        while most_splits and -(-max_pages // pages_per_split) > most_splits:
             pages_per_split *= 2
     return pages_per_split, max(1, -(-max_pages // pages_per_split))
 
@@ -579,7 +586,7 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
         pre = groups.splits(total_suffix_pages)
         tail = tail_split_plan(groups.batch, groups.q_heads, groups.kv_heads,
                                max_suffix_pages or block_table.shape[1], pages_per_split,
-                               total_suffix_pages, sms or groups.sms)
+                               total_suffix_pages, sms or groups.sms, MOST_PARTS - pre[1])
         done = fast.shared_prefix_attention(
             q, kv_pool, block_table, ctx_len, scale, out, lse_out, groups.packed, pre, tail,
             workspace.parts(groups.batch * groups.q_heads, groups.head_dim, pre[1], tail[1]))
@@ -609,9 +616,9 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
                                       max_pages_in_batch=max_suffix_pages,
                                       total_pages=total_suffix_pages, out=out, lse_out=lse_out,
                                       sms=sms)
-    pps, nsplit = tail_split_plan(B, hq, hkv, max_suffix_pages or max_pages, pages_per_split,
-                                  total_suffix_pages, sms or groups.sms)
     pre_pps, pre_splits = groups.splits(total_suffix_pages)
+    pps, nsplit = tail_split_plan(B, hq, hkv, max_suffix_pages or max_pages, pages_per_split,
+                                  total_suffix_pages, sms or groups.sms, MOST_PARTS - pre_splits)
     if out is None:
         out = q.new_empty((B, hq, dim))
     else:

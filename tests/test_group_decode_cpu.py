@@ -161,3 +161,16 @@ def test_freed_by_counts_pages_that_nobody_else_owns():
     c = blocks.adopt("c", shared + blocks.take_pages(1), 40)
     for slots, pages in (([a], 1), ([b], 2), ([c], 1), ([a, c], 4), ([a, b, c], 6), ([], 0)):
         assert blocks.freed_by(slots) == pages
+
+
+@pytest.mark.parametrize("kv_heads", [1, 2, 8])
+@pytest.mark.parametrize("prefix_splits", [1, 37, 148])
+def test_tail_split_plan_keeps_to_the_parts_that_the_entry_takes(kv_heads, prefix_splits):
+    """Own pages of 64k to 5M tokens, with and without their number known."""
+    most = paged.MOST_PARTS - prefix_splits
+    for pages in (4000, 4079, 4080, 4200, 4735, 8200, 9471, 16300, 18750, 65536, 327680):
+        for batch, total in ((1, pages), (2, pages + 3), (64, pages + 640), (8, None)):
+            pps, splits = paged.tail_split_plan(batch, 16, kv_heads, pages, None, total, 148, most)
+            assert splits <= most and pps * splits >= pages > pps * (splits - 1)
+            free = paged.tail_split_plan(batch, 16, kv_heads, pages, None, total, 148)
+            assert free == (pps, splits) or free[1] > most

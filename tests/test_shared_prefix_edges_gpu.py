@@ -187,3 +187,18 @@ def test_tokens_with_scores_of_minus_infinity_weigh_nothing(cuda, hq, hkv, D):
     _check(cuda, case)
     for splits in (1, 2, 8):
         _check(cuda, case, pages_per_split=splits)
+
+
+@pytest.mark.parametrize("hq,hkv,D", [(16, 2, 256), (6, 1, 128), (8, 8, 64)])
+@pytest.mark.parametrize("pages_per_split", [31, 32, 33, 64, 100])
+def test_units_of_more_pages_than_a_warp_has_lanes(cuda, hq, hkv, D, pages_per_split):
+    case = _case(cuda, [(2, 48), (2, 160)], [40 * 16, 1, 33 * 16, 66 * 16 + 5], hq, hkv, D, seed=13,
+                 single=[130 * 16 - 3, 20])
+    _check(cuda, case, pages_per_split=pages_per_split)
+
+
+@pytest.mark.parametrize("tokens,hint", [(70_000, True), (70_000, False), (290_000, True)])
+def test_a_long_sequence_beside_a_group(cuda, tokens, hint):
+    """One kv head: more parts of 4, 8 or 16 pages than the entry point takes, so longer ones."""
+    case = _case(cuda, [(2, 64)], [5, 30], 4, 1, 64, seed=14, single=[tokens])
+    _check(cuda, case, hint=hint)
