@@ -454,8 +454,10 @@ class PrefixGroups:
         # Two splits of the prefix: where it is most of the work, and where the sequences'
         # own pages are a good part of it (see splits()).
         self.sms = sms = sms or sm_count(device)
+        self.most_splits = most_splits(batch * q_heads, head_dim)
         self._splits = [prefix_split_plan([t[2] for t in tiles], kv_heads, head_dim, n,
-                                          pages_per_split) for n in (sms, max(1, sms * 7 // 9))]
+                                          pages_per_split, self.most_splits)
+                        for n in (sms, max(1, sms * 7 // 9))]
         # One transfer: tiles [ntiles, 4], then first_page [batch], then members.
         flat = torch.tensor([x for t in tiles for x in t] + first_page + members,
                             dtype=torch.int32).to(device)
@@ -481,10 +483,10 @@ class PrefixGroups:
 
 
 def prefix_split_plan(tile_pages: list, kv_heads: int, head_dim: int, sms: int,
-                      pages_per_split: int | None = None) -> tuple:
+                      pages_per_split: int | None = None, most: int | None = None) -> tuple:
     """(pages_per_split, num_splits) of the shared pages, in whole tiles of the kernel (4
     pages at D = 256, else 8): as many equal splits as give at most one CTA per SM over
-    all tiles and kv heads."""
+    all tiles and kv heads, and at most `most`."""
     unit = 4 if head_dim == 256 else 8
     longest = max(tile_pages, default=1)
     if not pages_per_split:
@@ -493,28 +495,40 @@ def prefix_split_plan(tile_pages: list, kv_heads: int, head_dim: int, sms: int,
         ctas = lambda p: sum(-(-t // p) for t in tile_pages) * kv_heads  # noqa: E731
         while ctas(pages_per_split) > sms and pages_per_split < longest:
             pages_per_split += unit
+        if most:
+            pages_per_split = max(pages_per_split, -(-longest // most))
     pps = -(-pages_per_split // unit) * unit
     return pps, max(1, -(-longest // pps))
 
 
-MOST_PARTS = 1024  # parts of one (row, head) that the merge takes
+MOST_PARTS = 1024      # parts of one (row, head) that the merge takes
+PART_BYTES = 256 << 20  # of scratch for the prefixes' parts, and for the own pages'
+
+
+def most_splits(rows: int, head_dim: int) -> int:
+    """Splits whose parts fit PART_BYTES, eight at least: every (row, head) has room for as
+    many parts as the longest sequence needs, so one long sequence in a large batch would
+    otherwise ask for gigabytes. 256 sequences (16 heads of 256), one of them with 131,072 own
+    tokens: 0.28 GB and 148 us, with units of 16 pages 2.17 GB and 188 us; with 32,768 own
+    tokens 0.28 GB and 68 us, 0.55 GB and 71 us."""
+    return max(8, PART_BYTES // (4 * head_dim * max(1, rows)))
 
 
 def tail_split_plan(batch: int, q_heads: int, kv_heads: int, max_pages: int,
                     pages_per_split: int | None, total_pages: int | None, sms: int,
-                    most_splits: int | None = None) -> tuple:
+                    most: int | None = None) -> tuple:
     """(pages_per_split, num_splits) of the sequences' own pages beside a prefix: units of
     work of up to 16 pages, small enough that every warp of two CTAs an SM gets some. 64
     sequences of U[1, 2048] tokens took 35.5 / 32.1 / 31.2 / 36.3 us in units of 4 / 8 / 16 /
     32 pages, 15 of U[1, 777] 13.5 / 13.4 / 17.3 / 26.8. Units double on where the longest
-    sequence would have more than most_splits of them (a limit, not a matter of speed)."""
+    sequence would have more than `most` of them (a limit, not a matter of speed)."""
     if not pages_per_split:
         groups = kv_heads * ((q_heads // kv_heads + 7) // 8)
         work = (total_pages or batch * max_pages) * groups
         pages_per_split = 4
         while pages_per_split < 16 and work / (2 * pages_per_split) >= 4 * sms:
             pages_per_split *= 2
-        while most_splits and -(-max_pages // pages_per_split) > most_splits:
+        while most and -(-max_pages // pages_per_split) > most:
             pages_per_split *= 2
     return pages_per_split, max(1, -(-max_pages // pages_per_split))
 
@@ -586,7 +600,8 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
         pre = groups.splits(total_suffix_pages)
         tail = tail_split_plan(groups.batch, groups.q_heads, groups.kv_heads,
                                max_suffix_pages or block_table.shape[1], pages_per_split,
-                               total_suffix_pages, sms or groups.sms, MOST_PARTS - pre[1])
+                               total_suffix_pages, sms or groups.sms,
+                               min(MOST_PARTS - pre[1], groups.most_splits))
         done = fast.shared_prefix_attention(
             q, kv_pool, block_table, ctx_len, scale, out, lse_out, groups.packed, pre, tail,
             workspace.parts(groups.batch * groups.q_heads, groups.head_dim, pre[1], tail[1]))
@@ -618,7 +633,8 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
                                       sms=sms)
     pre_pps, pre_splits = groups.splits(total_suffix_pages)
     pps, nsplit = tail_split_plan(B, hq, hkv, max_suffix_pages or max_pages, pages_per_split,
-                                  total_suffix_pages, sms or groups.sms, MOST_PARTS - pre_splits)
+                                  total_suffix_pages, sms or groups.sms,
+                                  min(MOST_PARTS - pre_splits, groups.most_splits))
     if out is None:
         out = q.new_empty((B, hq, dim))
     else:

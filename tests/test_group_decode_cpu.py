@@ -174,3 +174,19 @@ def test_tail_split_plan_keeps_to_the_parts_that_the_entry_takes(kv_heads, prefi
             assert splits <= most and pps * splits >= pages > pps * (splits - 1)
             free = paged.tail_split_plan(batch, 16, kv_heads, pages, None, total, 148)
             assert free == (pps, splits) or free[1] > most
+
+
+@pytest.mark.parametrize("batch", [2, 64, 256, 1024, 5000])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (16, 1, 256), (32, 8, 128), (8, 8, 64)])
+def test_parts_of_one_long_sequence_in_a_large_batch_stay_small(batch, heads, kv_heads, dim):
+    """Two rows on a long prefix, one row of 128k own tokens, the others short."""
+    groups = paged.PrefixGroups([([0, 1], 200_000)], batch, heads, kv_heads, dim, device="cpu",
+                                sms=148)
+    part = 4 * batch * heads * dim
+    most = max(paged.PART_BYTES, 8 * part)
+    for own in (None, batch + 8192):
+        pps, splits = groups.splits(own)
+        assert splits * part <= most and pps * splits >= 12500 > pps * (splits - 1)
+        pps, splits = paged.tail_split_plan(batch, heads, kv_heads, 8192, None, own, 148,
+                                            groups.most_splits)
+        assert splits * part <= most and pps * splits >= 8192 > pps * (splits - 1)
