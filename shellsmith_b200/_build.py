@@ -7,6 +7,7 @@ import os
 import shutil
 import subprocess
 import sysconfig
+import warnings
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -36,27 +37,36 @@ def _stale() -> bool:
 
 
 def _build_fastpath(force: bool, verbose: bool) -> None:
-    """Compile the callers (csrc/fastpath.cpp) against torch; they link the library."""
+    """Compile the callers (csrc/fastpath.cpp) against torch; they link the library. They are
+    optional: where g++, torch or Python's headers are missing, a warning says so, callers of
+    an older build are removed, and the Python wrappers make the calls."""
     inputs = [CSRC / "fastpath.cpp", PACKAGE.parent / "include" / "shellcache.h"]
     if not force and FASTPATH.exists() and all(p.stat().st_mtime <= FASTPATH.stat().st_mtime
                                                for p in inputs):
         return
-    import torch
-
-    base = Path(torch.__file__).resolve().parent
-    cuda = Path(nvcc()).resolve().parent.parent
     tmp = FASTPATH.with_suffix(".so.tmp")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f"-I{base}/include", f"-I{base}/include/torch/csrc/api/include",
-           f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", str(inputs[0]),
-           "-o", str(tmp), f"-L{PACKAGE}", "-l:libshellcache.so", f"-L{base}/lib", "-lc10",
-           "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
-    if verbose:
-        print(" ".join(cmd))
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stderr[-4000:]}")
+    try:
+        import torch
+
+        base = Path(torch.__file__).resolve().parent
+        cuda = Path(nvcc()).resolve().parent.parent
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f"-I{base}/include", f"-I{base}/include/torch/csrc/api/include",
+               f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", str(inputs[0]),
+               "-o", str(tmp), f"-L{PACKAGE}", "-l:libshellcache.so", f"-L{base}/lib", "-lc10",
+               "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+        if verbose:
+            print(" ".join(cmd))
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        failed = f"g++ failed ({proc.returncode}):\n{proc.stderr[-4000:]}" if proc.returncode else None
+    except (ImportError, OSError) as err:
+        failed = f"{type(err).__name__}: {err}"
+    if failed is not None:
+        FASTPATH.unlink(missing_ok=True)
+        warnings.warn(f"the group-decode operators' compiled callers are not built, their Python "
+                      f"wrappers will be used: {failed}", stacklevel=2)
+        return
     os.replace(tmp, FASTPATH)
 
 
