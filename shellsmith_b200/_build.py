@@ -38,7 +38,7 @@ def _stale() -> bool:
 
 def _build_fastpath(force: bool, verbose: bool) -> None:
     """Compile the callers (csrc/fastpath.cpp) against torch; they link the library. They are
-    optional: where g++, torch or Python's headers are missing, a warning says so, callers of
+    optional: where g++, torch, its CUDA headers or Python's are missing, a warning says so, callers of
     an older build are removed, and the Python wrappers make the calls."""
     inputs = [CSRC / "fastpath.cpp", PACKAGE.parent / "include" / "shellcache.h"]
     if not force and FASTPATH.exists() and all(p.stat().st_mtime <= FASTPATH.stat().st_mtime
@@ -60,7 +60,7 @@ def _build_fastpath(force: bool, verbose: bool) -> None:
             print(" ".join(cmd))
         proc = subprocess.run(cmd, capture_output=True, text=True)
         failed = f"g++ failed ({proc.returncode}):\n{proc.stderr[-4000:]}" if proc.returncode else None
-    except (ImportError, OSError) as err:
+    except (ImportError, OSError, RuntimeError) as err:  # RuntimeError: no CUDA toolkit
         failed = f"{type(err).__name__}: {err}"
     if failed is not None:
         FASTPATH.unlink(missing_ok=True)

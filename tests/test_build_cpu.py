@@ -48,3 +48,12 @@ def test_up_to_date_callers_stay(callers, monkeypatch):
     monkeypatch.setattr(_build.subprocess, "run", lambda *a, **kw: pytest.fail("compiled"))
     assert _build.build() == _build.LIBRARY
     assert callers.read_bytes() == b"old"
+
+
+def test_a_built_library_needs_no_toolkit(callers, monkeypatch):
+    def missing():
+        raise RuntimeError("nvcc not found")
+    monkeypatch.setattr(_build, "nvcc", missing)
+    with pytest.warns(UserWarning, match="nvcc not found"):
+        assert _build.build() == _build.LIBRARY
+    assert not callers.exists()
