@@ -40,7 +40,7 @@ def _build_fastpath(force: bool, verbose: bool) -> None:
     """Compile the callers (csrc/fastpath.cpp) against torch; they link the library. They are
     optional: where g++, torch, its CUDA headers or Python's are missing, a warning says so, callers of
     an older build are removed, and the Python wrappers make the calls."""
-    inputs = [CSRC / "fastpath.cpp", PACKAGE.parent / "include" / "shellcache.h"]
+    inputs = [CSRC / "fastpath.cpp", PACKAGE.parent / "include" / "shellcache.h", Path(__file__)]
     if not force and FASTPATH.exists() and all(p.stat().st_mtime <= FASTPATH.stat().st_mtime
                                                for p in inputs):
         return
@@ -52,6 +52,7 @@ def _build_fastpath(force: bool, verbose: bool) -> None:
         cuda = Path(nvcc()).resolve().parent.parent
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f'-DSC_TORCH_VERSION="{torch.__version__}"',
                f"-I{base}/include", f"-I{base}/include/torch/csrc/api/include",
                f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", str(inputs[0]),
                "-o", str(tmp), f"-L{PACKAGE}", "-l:libshellcache.so", f"-L{base}/lib", "-lc10",

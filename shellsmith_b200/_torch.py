@@ -21,9 +21,12 @@ def stream_of(t: torch.Tensor) -> int:
 
 
 # The compiled callers of the group-decode operators (csrc/fastpath.cpp), or None where
-# they are not built: the wrappers then make the same calls themselves.
+# they are not built, or built for another torch: the wrappers then make the same calls
+# themselves.
 try:
     from . import _fastpath as fast
+    if getattr(fast, "torch_version", None) != torch.__version__:
+        fast = None
 except ImportError:
     fast = None
 

@@ -249,4 +249,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastpath", nullptr, -1, methods};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fastpath() { return PyModule_Create(&module); }
+// The module reaches into torch's C++ objects: with another torch than it was compiled for it
+// must not be used, even where it links.
+PyMODINIT_FUNC PyInit__fastpath() {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "torch_version", SC_TORCH_VERSION) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -1,11 +1,13 @@
 """The build without what only the compiled callers need: the library is all that counts."""
 
+import importlib
 import subprocess
 import sys
 
 import pytest
+import torch
 
-from shellsmith_b200 import _build
+from shellsmith_b200 import _build, _torch
 
 
 @pytest.fixture
@@ -57,3 +59,15 @@ def test_a_built_library_needs_no_toolkit(callers, monkeypatch):
     with pytest.warns(UserWarning, match="nvcc not found"):
         assert _build.build() == _build.LIBRARY
     assert not callers.exists()
+
+
+def test_callers_of_another_torch_are_not_used(monkeypatch):
+    if _torch.fast is None:
+        pytest.skip("the compiled callers are not built")
+    assert _torch.fast.torch_version == torch.__version__
+    try:
+        with monkeypatch.context() as m:
+            m.setattr(torch, "__version__", "0.0.1")
+            assert importlib.reload(_torch).fast is None
+    finally:
+        assert importlib.reload(_torch).fast is not None
