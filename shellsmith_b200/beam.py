@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 
 import numpy as np
 import torch
@@ -59,6 +60,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, *,
     fp32 = logits.dtype is torch.float32
     if not fp32 and logits.dtype is not torch.bfloat16:
         raise TypeError(f"logits must be bfloat16 or float32, got {logits.dtype}")
+    for name, value in (("n", n), ("pad_token", pad_token)):
+        if not -1 << 31 <= operator.index(value) < 1 << 31:  # it would wrap on its way
+            raise ValueError(f"beam_select: {name}={value} does not fit 32 bits")
+    if n < 0:
+        raise ValueError(f"beam_select: n={n}")
     groups, beams, vocab = logits.shape
     if beams < 1 or vocab < 1:
         raise ValueError("beam_select: at least one beam and one token")

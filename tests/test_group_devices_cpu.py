@@ -124,3 +124,20 @@ def test_shared_prefix_attention(launched, monkeypatch, rows):
         with pytest.raises(ValueError):
             paged.shared_prefix_attention(scale=0.1, groups=groups, workspace=other, **operands)
         assert len(launched) == 1
+
+
+def test_beam_select_refuses_numbers_that_do_not_fit(launched, monkeypatch):
+    """2^32 + 2 tokens from the pad token's place would be token 2 in the C call."""
+    monkeypatch.setattr(beam, "_workspace", lambda *a: 256)
+    x, s = _bf(2, 3, 50), on(torch.zeros((2, 3)))
+    done = on(torch.zeros((2, 3), dtype=torch.bool))
+    for pad in (2 ** 32 + 2, 2 ** 31, -2 ** 31 - 1):
+        with pytest.raises(ValueError):
+            beam.beam_select(x, s, 4, finished=done, pad_token=pad)
+    for n in (2 ** 32 + 4, -1, -2 ** 40):
+        with pytest.raises(ValueError):
+            beam.beam_select(x, s, n)
+    for n in (4.0, "4", None):
+        with pytest.raises(TypeError):
+            beam.beam_select(x, s, n)
+    assert not launched
