@@ -555,7 +555,7 @@ int sc_shared_prefix_attention(const sc_bf16* q, const sc_bf16* kv_pool, int64_t
  * out_scores, parents, tokens [groups, n]; where fewer than n scores are above
  *               -inf, the entries of lowest index follow with -inf
  * workspace     sc_beam_select_workspace bytes, 256-byte aligned
- * Supported: beams <= 64, n <= 64, beams * vocab < 2^31, groups * beams <= 65535. */
+ * Supported: beams <= 64, n <= 64, beams * vocab <= 2^31 - 2^14, groups * beams <= 65535. */
 size_t sc_beam_select_workspace(int groups, int beams, int vocab, int n, int logits_fp32);
 int sc_beam_select(const void* logits, int logits_fp32, int64_t row_stride, const float* scores,
                    const uint8_t* finished, int pad_token, float* out_scores, int32_t* parents,

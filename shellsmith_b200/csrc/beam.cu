@@ -982,8 +982,9 @@ extern "C" int sc_beam_select(const void* logits, int logits_fp32, int64_t row_s
              (long long)row_stride);
   SC_REQUIRE(beams <= sc::kMaxBeams, SC_ERR_UNSUPPORTED, "%s: %d beams, at most %d", name, beams,
              sc::kMaxBeams);
-  SC_REQUIRE((long long)beams * vocab < (1ll << 31), SC_ERR_UNSUPPORTED,
-             "%s: beams * vocab = %lld does not fit 31 bits", name, (long long)beams * vocab);
+  // Indices are 32-bit; the scan looks up to two rounds of blocks past a row's end for them.
+  SC_REQUIRE((long long)beams * vocab <= (1ll << 31) - (1ll << 14), SC_ERR_UNSUPPORTED,
+             "%s: beams * vocab = %lld, at most 2^31 - 2^14", name, (long long)beams * vocab);
   SC_REQUIRE(n > 0 && n <= sc::kMaxSelect && n <= (long long)beams * vocab, SC_ERR_UNSUPPORTED,
              "%s: n=%d not in 1..min(%d, beams * vocab)", name, n, sc::kMaxSelect);
   SC_REQUIRE(finished == nullptr || (pad_token >= 0 && pad_token < vocab), SC_ERR_INVALID,

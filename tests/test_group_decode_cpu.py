@@ -1,11 +1,13 @@
 """Host logic of group decode (no GPU): plans, page bookkeeping, operator registration."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from shellsmith_b200 import beam, paged, rotary, torch_ops
+from shellsmith_b200 import _capi, beam, paged, rotary, torch_ops
 from shellsmith_b200.block_manager import BlockManager
 
 
@@ -190,3 +192,15 @@ def test_parts_of_one_long_sequence_in_a_large_batch_stay_small(batch, heads, kv
         pps, splits = paged.tail_split_plan(batch, heads, kv_heads, 8192, None, own, 148,
                                             groups.most_splits)
         assert splits * part <= most and pps * splits >= 8192 > pps * (splits - 1)
+
+
+@pytest.mark.parametrize("beams,vocab", [(1, 2 ** 31 - 1), (1, 2 ** 31 - 2 ** 14 + 1), (2, 2 ** 30),
+                                         (64, 2 ** 25 + 1)])
+def test_beam_select_refuses_more_than_its_indices_hold(beams, vocab):
+    """Refused by the entry point before it looks at the memory or the GPU."""
+    unsupported = 2
+    host = ctypes.create_string_buffer(512)
+    at = (ctypes.addressof(host) + 255) // 256 * 256
+    code = _capi.lib().sc_beam_select(at, 0, vocab, at, None, 0, at, at, at, at, 2 ** 60, 1, beams,
+                                      vocab, 4, None)
+    assert code == unsupported and "beams * vocab" in _capi.last_error()
