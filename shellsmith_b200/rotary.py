@@ -165,16 +165,16 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     if k_shape[1] != hkv or k_shape[2] != dim or slot_mapping.shape[0] != k_shape[0]:
         raise ValueError("rotary_append: k/v must be [ntok, Hkv, D] with one slot per token")
     on_device(plan.device_index, v=v, kv_pool=kv_pool, slot_mapping=slot_mapping, out=out)
+    if out is not None:
+        require_cuda("out", out, torch.bfloat16, 3)
+        if out.shape != q_shape:
+            raise ValueError("rotary_append: out must have q's shape")
     if kv_pool.dtype is torch.uint8:
         q_out, k_out = rotary(q, k, positions, plan, q_weight=q_weight, k_weight=k_weight, eps=eps)
         paged.kv_append(k_out, v.contiguous(), kv_pool, slot_mapping)
         return q_out if out is None else out.copy_(q_out)
     if out is None:
         out = q.new_empty(q_shape)
-    else:
-        require_cuda("out", out, torch.bfloat16, 3)
-        if out.shape != q_shape:
-            raise ValueError("rotary_append: out must have q's shape")
     _run(q, k, v.data_ptr(), k_shape, (qs[0], qs[1], ks[0], ks[1], vs[0], vs[1]), positions, plan,
          q_weight, k_weight, eps, out, None, kv_pool.data_ptr(), slot_mapping.data_ptr(), page,
          pages)

@@ -141,3 +141,21 @@ def test_beam_select_refuses_numbers_that_do_not_fit(launched, monkeypatch):
         with pytest.raises(TypeError):
             beam.beam_select(x, s, n)
     assert not launched
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_rotary_append_refuses_another_out(launched, monkeypatch, bits):
+    """Of 8-bit pools too, whose q is copied to out: one token would be spread over a larger
+    one, and rounded or widened into another type."""
+    monkeypatch.setattr(paged, "kv_append", lambda *a: launched.append("kv_append"))
+    plan = _plan(rotary.RotaryPlan, 128)
+    pool = on(torch.zeros((4, 1, 34 * 128), dtype=torch.uint8)) if bits == 8 else _bf(4, 1, 2, 16, 128)
+    args = (_bf(1, 2, 128), _bf(1, 1, 128), _bf(1, 1, 128), on(torch.zeros((1, 1), dtype=torch.int32)),
+            plan, pool, on(torch.zeros(1, dtype=torch.int64)))
+    for out in (_bf(5, 2, 128), _bf(1, 2, 64), _bf(2, 128), _bf(1, 128, 2).transpose(1, 2),
+                on(torch.zeros((1, 2, 128)))):
+        with pytest.raises((ValueError, TypeError)):
+            rotary.rotary_append(*args, out=out)
+        assert not launched
+    out = _bf(1, 2, 128)
+    assert rotary.rotary_append(*args, out=out) is out and launched
