@@ -161,7 +161,8 @@ class HybridCacheEngine:
         self.total_pages = 0
         self._group_ws = paged.SharedPrefixWorkspace(dev)
         self._groups = None           # PrefixGroups of the batch, for ...
-        self._groups_for = None       # ... this state of the block manager
+        self._groups_for = None       # ... these staged rows and pages
+        self._staged_sharing = None   # BlockManager.sharing when the step was staged
         self.rows = cfg.max_seqs  # rows the step's kernels cover (set by begin_step)
 
     # ------------------------------------------------------------ lifecycle
@@ -385,6 +386,7 @@ class HybridCacheEngine:
         self.rows = blocks.highest_active()
         self.max_pages_in_batch = max(1, int(blocks.pages_for(ctx.max())))
         self.total_pages = int(np.ceil(blocks.lengths[active] / self.cfg.page_size).sum())
+        self._staged_sharing = blocks.sharing
         self._d_stage.copy_(self._h_stage, non_blocking=True)  # every table at once
         self._staged.record()
         return len(active)
@@ -475,18 +477,22 @@ class HybridCacheEngine:
 
     def prefix_groups(self) -> paged.PrefixGroups:
         """The staged batch's sequences that share leading pages, laid out for
-        group_attention_layer; made anew when sequences come, go or change places."""
-        now = (self.rows, self.blocks.sharing)
-        if self._groups_for != now:
-            shared = [(slots, pages * self.cfg.page_size)
-                      for slots, pages in self.blocks.common_prefixes()]
+        group_attention_layer; made anew when sequences come, go or change places. Where
+        some did after begin_step, and nothing was laid out before, no group: the device's
+        tables are those that were staged."""
+        now = (self.rows, self._staged_sharing)
+        if self._groups_for != now or now[1] is None:
+            shared = []
+            if now[1] in (None, self.blocks.sharing):
+                shared = [(slots, pages * self.cfg.page_size)
+                          for slots, pages in self.blocks.common_prefixes()]
             self._groups = paged.PrefixGroups(shared, self.rows, self.cfg.q_heads,
                                               self.cfg.kv_heads, self.cfg.head_dim,
                                               device=self.device, sms=self.cfg.sms)
             self._groups_for = now
             first = np.zeros(self.rows, np.int64)
-            for slots, pages in shared:
-                first[slots] = pages
+            for slots, tokens in shared:
+                first[slots] = tokens // self.cfg.page_size
             self._first_page = first
         return self._groups
 

@@ -8,6 +8,7 @@ import pytest
 import torch
 from test_group_decode_gpu import _cfg, _search
 
+from shellsmith_b200 import _capi, paged
 from shellsmith_b200.block_manager import OutOfPages
 from shellsmith_b200.engine import HybridCacheEngine
 from shellsmith_b200.resident import ToyHybridModel
@@ -111,3 +112,37 @@ def test_reorder_takes_the_pages_that_its_beams_give_back(cuda):
         for i in range(2):
             assert torch.equal(eng.kv[:, mine[i]], kv[:, pages[p][i]])
     assert eng.blocks.free_pages == 2     # two full pages went, the partial ones came back
+
+
+@pytest.mark.parametrize("laid_out", [False, True])
+@pytest.mark.parametrize("low_slot", [False, True])
+def test_sequences_that_come_between_staging_and_attention(cuda, laid_out, low_slot):
+    """A fork after begin_step, into a slot past the staged rows or below them: the staged rows
+    attend to what was staged (a lower slot would lead the group with a table row that the
+    device does not have)."""
+    cfg = _cfg()
+    eng = HybridCacheEngine(cfg, device=cuda)
+    first = eng.admit("first", 40)        # holds slot 0
+    a = eng.admit("a", 100)
+    eng.kv.copy_(torch.randn(eng.kv.shape, device=cuda).to(torch.bfloat16))
+    snap = eng.snapshot(a)
+    for _ in range(2):
+        eng.fork(snap)
+    if low_slot:
+        eng.release(first)
+    eng.begin_step()
+    if laid_out:
+        assert eng.prefix_groups().ntiles == 1
+    new = eng.fork(snap)
+    assert new == (0 if low_slot else eng.rows)
+    n, layer = eng.rows, cfg.attention_layers[0]
+    q = torch.randn((n, cfg.q_heads, cfg.head_dim), device=cuda).to(torch.bfloat16)
+    out = torch.empty_like(q)
+    eng.group_attention_layer(layer, q, out)
+    want = paged.paged_decode_attention(q, eng.kv[eng.attn_index[layer]], eng.table[:n],
+                                        eng.ctx_len[:n], eng.scale)
+    _capi.check_device()
+    # Both round P to bf16 in other places: 2^-8 of sum p |v| (below 2) each, and the output.
+    assert (out.float() - want.float()).abs().max() <= 3 * 2.0 ** -8 * 2
+    eng.begin_step()
+    assert eng.prefix_groups().ntiles == 1 and len(eng.prefix_groups().members) == 4
