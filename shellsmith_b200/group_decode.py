@@ -168,6 +168,8 @@ class BeamSearch:
 
     def search(self, prompt: list, beams: int, max_tokens: int) -> list:
         """The best continuations of the prompt, up to max_tokens long, best first."""
+        if max_tokens < 1:
+            raise ValueError(f"search: max_tokens={max_tokens}, the prompt gives one at least")
         self.start(prompt, beams)
         while len(max(self.beams, key=lambda b: len(b.tokens)).tokens) < max_tokens and self.step():
             pass

@@ -146,3 +146,13 @@ def test_sequences_that_come_between_staging_and_attention(cuda, laid_out, low_s
     assert (out.float() - want.float()).abs().max() <= 3 * 2.0 ** -8 * 2
     eng.begin_step()
     assert eng.prefix_groups().ntiles == 1 and len(eng.prefix_groups().members) == 4
+
+
+def test_search_refuses_less_than_a_token(cuda):
+    cfg = _cfg()
+    eng, search = _search(cuda, cfg, ToyHybridModel(cfg, device=cuda))
+    for count in (0, -3):
+        with pytest.raises(ValueError):
+            search.search([1, 2, 3], 2, count)
+    assert not search.slots
+    assert all(len(b.tokens) == 1 for b in search.search([1, 2, 3], 2, 1))
