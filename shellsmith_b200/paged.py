@@ -465,11 +465,18 @@ class PrefixGroups:
         self.first_page = flat[4 * len(tiles):4 * len(tiles) + batch]
         self.members = flat[4 * len(tiles) + batch:]
         self.device_index = flat.get_device()
+        self._tables, self._home = flat, stream_of(flat) if flat.is_cuda else 0
         self.tiles_ptr, self.first_page_ptr, self.members_ptr = (
             flat.data_ptr() + 4 * n for n in (0, 4 * len(tiles), 4 * len(tiles) + batch))
         self.packed = (batch, q_heads, kv_heads, head_dim, self.device_index, self.ntiles,
                        self.max_prefix_pages, self.first_page_ptr, self.tiles_ptr,
                        self.members_ptr)
+
+    def used(self) -> None:
+        """A call on the current stream reads the tables: if they came from another stream, the
+        allocator does not hand their memory out before the call is done."""
+        if stream_of(self._tables) != self._home:
+            self._tables.record_stream(torch.cuda.current_stream(self.device_index))
 
     def splits(self, own_pages: int | None) -> tuple:
         """(pages_per_split, num_splits) of the shared pages beside `own_pages` pages of the
@@ -596,6 +603,8 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
     if workspace is not None and workspace.device_index != groups.device_index:
         raise ValueError(f"the workspace is on {workspace.device}, the groups on "
                          f"{groups.tiles.device}")
+    if groups.ntiles:
+        groups.used()
     if fast is not None and workspace is not None and groups.ntiles:
         pre = groups.splits(total_suffix_pages)
         tail = tail_split_plan(groups.batch, groups.q_heads, groups.kv_heads,
