@@ -130,7 +130,9 @@ def reorder_rows(pools, slots: torch.Tensor, parents: torch.Tensor) -> torch.Ten
         sizes[i] = pool.stride(1) * pool.element_size()
     on_device(slots.get_device(), parents=parents, **{f"pool {i}": p for i, p in enumerate(pools)})
     out = torch.empty_like(slots)
-    _reorder(bases, sizes, layers, count, rows or 1, slots.data_ptr(), parents.data_ptr(),
+    if rows is None:  # the new slots alone: any slot is in range
+        rows = (1 << 31) - 1
+    _reorder(bases, sizes, layers, count, rows, slots.data_ptr(), parents.data_ptr(),
              out.data_ptr(), groups, beams or 1, stream_of(slots))
     return out
 

@@ -73,3 +73,18 @@ def test_tile_after_a_list_that_is_just_not_cut(cuda, dtype, left):
     x[first] = 2.0 + torch.arange(left, device=cuda) % 7 * 0.125
     for R in (1, 5, 700):
         _exact(x.to(dtype).expand(R, V).contiguous(), 64)
+
+
+def test_reorder_without_pools_flags_nothing(cuda):
+    """The new slots alone: no row is out of range where there is none."""
+    slots = torch.tensor([[4, 1, 0, 5]], dtype=torch.int32, device=cuda)
+    parents = torch.tensor([[2, 2, 0, 2]], dtype=torch.int32, device=cuda)
+    _capi.device_status()
+    assert beam.reorder_rows([], slots, parents).tolist() == [[0, 1, 4, 5]]
+    assert beam.reorder_rows((), slots, parents).tolist() == [[0, 1, 4, 5]]
+    _capi.check_device()
+    with pytest.raises(_capi.DeviceFault):
+        beam.reorder_rows([], slots, parents + 9)
+        _capi.check_device()
+    with pytest.raises(_capi.ShellcacheError):
+        beam.reorder_rows([torch.empty((2, 0, 8), device=cuda)], slots, parents)
