@@ -171,7 +171,9 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
             raise ValueError("rotary_append: out must have q's shape")
     if kv_pool.dtype is torch.uint8:
         q_out, k_out = rotary(q, k, positions, plan, q_weight=q_weight, k_weight=k_weight, eps=eps)
-        paged.kv_append(k_out, v.contiguous(), kv_pool, slot_mapping)
+        if not v.is_contiguous() or v.data_ptr() % 16:  # one token's view may be off a boundary
+            v = v.clone(memory_format=torch.contiguous_format)
+        paged.kv_append(k_out, v, kv_pool, slot_mapping)
         return q_out if out is None else out.copy_(q_out)
     if out is None:
         out = q.new_empty(q_shape)

@@ -159,3 +159,17 @@ def test_rotary_append_refuses_another_out(launched, monkeypatch, bits):
         assert not launched
     out = _bf(1, 2, 128)
     assert rotary.rotary_append(*args, out=out) is out and launched
+
+
+@pytest.mark.parametrize("first", [0, 1, 3, 8])
+def test_rotary_append_of_one_token_off_a_boundary_to_8_bit_pages(launched, monkeypatch, first):
+    """One token's view of v is contiguous wherever it starts; the append wants 16 bytes."""
+    taken = []
+    monkeypatch.setattr(paged, "kv_append", lambda k, v, *a: taken.append(v))
+    plan = _plan(rotary.RotaryPlan, 128)
+    v = on(torch.arange(140, dtype=torch.bfloat16)[first:first + 128].view(1, 1, 128))
+    rotary.rotary_append(_bf(1, 2, 128), _bf(1, 1, 128), v, on(torch.zeros((1, 1), dtype=torch.int32)),
+                         plan, on(torch.zeros((4, 1, 34 * 128), dtype=torch.uint8)),
+                         on(torch.zeros(1, dtype=torch.int64)))
+    assert taken[0].is_contiguous() and taken[0].data_ptr() % 16 == 0
+    assert torch.equal(taken[0].as_subclass(torch.Tensor), v.as_subclass(torch.Tensor))
