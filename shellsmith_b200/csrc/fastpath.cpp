@@ -38,7 +38,17 @@ bool dense(const at::Tensor* t, int device, at::ScalarType type, int64_t ndim, s
          t->dim() == ndim && t->is_contiguous() && aligned(*t, align);
 }
 
-void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
+// The current stream, on which a call reads a plan's tables (the tuple's items from `first` on).
+// If those came from another stream, the allocator does not hand their memory out before the
+// call is done.
+void* stream_of(int device, PyObject* plan = nullptr, Py_ssize_t first = 0, long long home = 0) {
+  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
+  if (plan != nullptr && reinterpret_cast<uintptr_t>(stream.stream()) != (uintptr_t)home)
+    for (Py_ssize_t i = first; i < PyTuple_GET_SIZE(plan); ++i)
+      if (THPVariable_Check(PyTuple_GET_ITEM(plan, i)))
+        THPVariable_Unpack(PyTuple_GET_ITEM(plan, i)).record_stream(stream.unwrap());
+  return stream.stream();
+}
 
 template <typename T>
 T* data(const at::Tensor* t) {
@@ -60,9 +70,9 @@ long long integer(PyObject* o, bool* ok) {
 long long item(PyObject* tuple, int i, bool* ok) { return integer(PyTuple_GET_ITEM(tuple, i), ok); }
 
 // rotary_append(q, k, v, positions, pool, slots, q_weight, k_weight, eps, out, plan): q
-// plan: (head_dim, rotary_dim, axes, turns, axis, device)
+// plan: (head_dim, rotary_dim, axes, turns, axis, device, home stream, its tables)
 PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) try {
-  if (n != 11 || !PyTuple_Check(a[10]) || PyTuple_GET_SIZE(a[10]) != 6) return none();
+  if (n != 11 || !PyTuple_Check(a[10]) || PyTuple_GET_SIZE(a[10]) != 9) return none();
   bool ok = true;
   const at::Tensor *q = tensor(a[0], &ok), *k = tensor(a[1], &ok), *v = tensor(a[2], &ok),
                    *pos = tensor(a[3], &ok), *pool = tensor(a[4], &ok), *slots = tensor(a[5], &ok),
@@ -75,6 +85,7 @@ PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) try {
   const long long dim = item(a[10], 0, &ok), rot = item(a[10], 1, &ok), axes = item(a[10], 2, &ok);
   const long long turns = item(a[10], 3, &ok), axis = item(a[10], 4, &ok);
   const int device = (int)item(a[10], 5, &ok);
+  const long long home = item(a[10], 6, &ok);
   if (!ok || q == nullptr || k == nullptr || v == nullptr || pos == nullptr) return none();
   for (const at::Tensor* t : {q, k, v})
     if (!t->is_cuda() || t->get_device() != device || t->scalar_type() != at::kBFloat16 ||
@@ -103,7 +114,8 @@ PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) try {
       flat ? 0 : pos->stride(0), (int)axes, reinterpret_cast<const double*>(turns),
       reinterpret_cast<const int32_t*>(axis), data<sc_bf16>(qw), data<sc_bf16>(kw), (float)eps,
       data<sc_bf16>(&fresh), nullptr, data<sc_bf16>(pool), data<int64_t>(slots), (int)ntok, (int)hq,
-      (int)hkv, (int)dim, (int)rot, (int)pool->size(3), pool->size(0), stream_of(device));
+      (int)hkv, (int)dim, (int)rot, (int)pool->size(3), pool->size(0),
+      stream_of(device, a[10], 7, home));
   return rc != 0 ? none() : THPVariable_Wrap(fresh);
 } catch (const std::exception&) {
   return none();
@@ -188,9 +200,10 @@ PyObject* reorder_rows(PyObject*, PyObject* const* a, Py_ssize_t n) try {
 // shared_prefix_attention(q, pool, table, ctx_len, scale, out, lse_out, groups, prefix_split,
 //                         tail_split, scratch): out
 // groups: (batch, q_heads, kv_heads, head_dim, device, ntiles, max_prefix_pages, first_page,
-// tiles, members); the splits are (pages, count); scratch the five addresses of the parts.
+// tiles, members, home stream, its tables); the splits are (pages, count); scratch the five
+// addresses of the parts.
 PyObject* shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) try {
-  if (n != 11 || !PyTuple_Check(a[7]) || PyTuple_GET_SIZE(a[7]) != 10) return none();
+  if (n != 11 || !PyTuple_Check(a[7]) || PyTuple_GET_SIZE(a[7]) != 12) return none();
   for (int i = 8; i < 11; ++i)
     if (!PyTuple_Check(a[i]) || PyTuple_GET_SIZE(a[i]) != (i < 10 ? 2 : 5)) return none();
   bool ok = true;
@@ -204,7 +217,7 @@ PyObject* shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) t
   const long long B = item(a[7], 0, &ok), hq = item(a[7], 1, &ok), hkv = item(a[7], 2, &ok),
                   dim = item(a[7], 3, &ok);
   const int device = (int)item(a[7], 4, &ok), ntiles = (int)item(a[7], 5, &ok);
-  const long long longest = item(a[7], 6, &ok);
+  const long long longest = item(a[7], 6, &ok), home = item(a[7], 10, &ok);
   long long at[3], part[5];
   for (int i = 0; i < 3; ++i) at[i] = item(a[7], 7 + i, &ok);
   for (int i = 0; i < 5; ++i) part[i] = item(a[10], i, &ok);
@@ -230,7 +243,7 @@ PyObject* shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) t
       pre_splits, pps, splits, (float)scale, reinterpret_cast<float*>(part[0]),
       reinterpret_cast<float*>(part[1]), reinterpret_cast<float*>(part[2]),
       reinterpret_cast<float*>(part[3]), reinterpret_cast<int32_t*>(part[4]), data<sc_bf16>(&fresh),
-      data<float>(lse), stream_of(device));
+      data<float>(lse), stream_of(device, a[7], 11, home));
   return rc != 0 ? none() : THPVariable_Wrap(fresh);
 } catch (const std::exception&) {
   return none();

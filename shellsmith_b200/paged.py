@@ -470,7 +470,7 @@ class PrefixGroups:
             flat.data_ptr() + 4 * n for n in (0, 4 * len(tiles), 4 * len(tiles) + batch))
         self.packed = (batch, q_heads, kv_heads, head_dim, self.device_index, self.ntiles,
                        self.max_prefix_pages, self.first_page_ptr, self.tiles_ptr,
-                       self.members_ptr)
+                       self.members_ptr, self._home, flat)
 
     def used(self) -> None:
         """A call on the current stream reads the tables: if they came from another stream, the
@@ -603,8 +603,6 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
     if workspace is not None and workspace.device_index != groups.device_index:
         raise ValueError(f"the workspace is on {workspace.device}, the groups on "
                          f"{groups.tiles.device}")
-    if groups.ntiles:
-        groups.used()
     if fast is not None and workspace is not None and groups.ntiles:
         pre = groups.splits(total_suffix_pages)
         tail = tail_split_plan(groups.batch, groups.q_heads, groups.kv_heads,
@@ -656,6 +654,7 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
             raise ValueError("shared_prefix_attention: lse_out must be [B * Hq]")
     if workspace is None:
         workspace = SharedPrefixWorkspace(q.device)
+    groups.used()
     _shared_prefix(q.data_ptr(), kv_pool.data_ptr(), num_pages, block_table.data_ptr(),
                    ctx_len.data_ptr(), groups.first_page_ptr, groups.tiles_ptr,
                    groups.members_ptr, groups.ntiles, B, hq, hkv, dim, page, max_pages, pre_pps,

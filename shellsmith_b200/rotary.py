@@ -58,8 +58,18 @@ class RotaryPlan:
         self.inv_freq = torch.tensor(inv_freq, dtype=torch.float64)
         self.turns = (self.inv_freq / (2 * math.pi)).to(device)  # whole turns per position
         self.device_index = self.turns.get_device()
+        self._home = stream_of(self.turns) if self.turns.is_cuda else 0
         self.turns_ptr, self.axis_ptr = self.turns.data_ptr(), self.axis.data_ptr()
-        self.packed = (head_dim, rot, self.axes, self.turns_ptr, self.axis_ptr, self.device_index)
+        self.packed = (head_dim, rot, self.axes, self.turns_ptr, self.axis_ptr, self.device_index,
+                       self._home, self.turns, self.axis)
+
+    def used(self) -> None:
+        """A call on the current stream reads the tables: if they came from another stream, the
+        allocator does not hand their memory out before the call is done."""
+        if stream_of(self.turns) != self._home:
+            stream = torch.cuda.current_stream(self.device_index)
+            self.turns.record_stream(stream)
+            self.axis.record_stream(stream)
 
 
 def axis_of_pairs(sections, interleaved: bool) -> list:
@@ -118,6 +128,7 @@ def _run(q, k, v, k_shape, strides, positions, plan, q_weight, k_weight, eps, q_
     if plan.device_index != q.get_device():
         raise ValueError(f"the plan is on {plan.turns.device}, q on {q.device}")
     on_device(plan.device_index, k=k, positions=positions, q_weight=q_weight, k_weight=k_weight)
+    plan.used()
     _append(q.data_ptr(), k.data_ptr(), v, _strides(*strides), positions.data_ptr(), pos_stride[0],
             plan.axes, plan.turns_ptr, plan.axis_ptr, _weight("q_weight", q_weight, dim),
             _weight("k_weight", k_weight, dim), eps, q_out.data_ptr(), k_out, pool, slots, ntok,

@@ -204,23 +204,30 @@ def test_a_long_sequence_beside_a_group(cuda, tokens, hint):
     _check(cuda, case, hint=hint)
 
 
-def test_groups_dropped_behind_queued_work(cuda):
+@pytest.mark.parametrize("compiled", [False, True])
+def test_groups_dropped_behind_queued_work(cuda, monkeypatch, compiled):
     """Groups laid out on one stream, used on another and dropped there at once: their tables'
     memory is not handed out while the call is still queued."""
     case = _case(cuda, [(3, 160), (4, 320)], [1, 9, 30, 4, 5, 6, 70], 16, 2, 256, seed=1)
     q, pool, table, ctx, plan = case
     t, c = torch.from_numpy(table).to(cuda), torch.from_numpy(ctx.astype(np.int32)).to(cuda)
+    ws = paged.SharedPrefixWorkspace(cuda)
+    _prepared(cuda, case, ws)()          # grown to its size
+    if not compiled:
+        monkeypatch.setattr(paged, "fast", None)
     groups = paged.PrefixGroups(plan, 7, 16, 2, 256, device=cuda)
     old, size = groups.tiles_ptr, groups.tiles.untyped_storage().nbytes()
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
         torch.cuda._sleep(200_000_000)
-        out = paged.shared_prefix_attention(q, pool, t, c, 0.0625, groups)
+        out = paged.shared_prefix_attention(q, pool, t, c, 0.0625, groups, workspace=ws)
     del groups
-    taken = [torch.full((size // 4,), -1, dtype=torch.int32, device=cuda) for _ in range(8)]
+    taken = [torch.empty((size // 4,), dtype=torch.int32, device=cuda) for _ in range(8)]
     assert old not in [x.data_ptr() for x in taken]
     assert not side.query()
+    for x in taken:
+        x.fill_(-1)
     torch.cuda.synchronize()
     _capi.check_device()
     _matches(out, case)
