@@ -207,8 +207,9 @@ class BlockManager:
         self.dirty_rows.add(slot)
 
     def common_prefixes(self) -> list:
-        """[(slots, pages)]: active sequences that start with the same pages, two at least,
-        with the number of leading pages that all of them share."""
+        """[(slots, pages)]: active sequences that start with the same page, two at least,
+        with the number of leading pages that all of them share (one that shares only the
+        first pages of a longer common prefix holds its group to those)."""
         by_first: dict = {}
         for slot in np.flatnonzero(self.active).tolist():
             if self.pages[slot]:

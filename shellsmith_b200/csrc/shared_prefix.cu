@@ -31,7 +31,10 @@
 // only when a row's maximum grows by more than 2^8 over its reference (until then P may
 // be as large as 2^8, which costs fp32 sums and bf16 P no accuracy).
 // P is rounded to bf16 for the tensor cores, as in the split-K kernel; scores, maxima,
-// sums and O are fp32. Two stages (128 KB at D = 256) leave room for the tail's CTA.
+// sums and O are fp32. The exponentials are ex2.approx here and __expf in the merge: a
+// few units in the last place, far below P's rounding. A row whose context ends inside the
+// prefix keeps its O from that page on: a page is a product, and a product can leave TMEM
+// lanes as they are. Two stages (128 KB at D = 256) leave room for the tail's CTA.
 //
 // tail_kernel. HBM-bound, 8 query heads to a K/V byte: the warp tensor path is enough.
 // Every warp is on its own: it takes a unit of work (a sequence, a kv head's group of up
@@ -43,13 +46,13 @@
 //
 // Measured (B200, 16 query over 2 kv heads of 256 unless said):
 //   8 groups of 8 sequences, prefixes of 16,272 and tails of U[1, 2048] tokens (402 MB)
-//     73.5 us, 5.5 TB/s, 83 % of a plain copy's rate: HBM, but for 5 us of start and 8 of
+//     73.9 us, 5.4 TB/s, 83 % of a plain copy's rate: HBM, but for 5 us of start and 8 of
 //     the last CTAs' parts and the merge
-//   128 sequences on 8,208 tokens, tails of U[1, 1024] (153 MB) 47.8 us: the prefix's eight
+//   128 sequences on 8,208 tokens, tails of U[1, 1024] (153 MB) 47.5 us: the prefix's eight
 //     tiles read it from the L2 and their products, the tails' loads and both softmaxes
 //     share the SMs for 40 us; the tails alone take 35
-//   3 groups of 5 on 5,104, tails of U[1, 777], 24 over 8 heads of 128 (87 MB) 24.0 us
-//   8 on 2,048, tails of U[1, 64] (5 MB) 12.3 us: the chain of three kernels (8 + 4 us)
+//   3 groups of 5 on 5,104, tails of U[1, 777], 24 over 8 heads of 128 (87 MB) 24.3 us
+//   8 on 2,048, tails of U[1, 64] (5 MB) 12.4 us: the chain of three kernels (8 + 4 us)
 #include <cudaTypedefs.h>
 #include <math_constants.h>
 
