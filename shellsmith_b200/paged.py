@@ -608,7 +608,7 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
         tail = tail_split_plan(groups.batch, groups.q_heads, groups.kv_heads,
                                max_suffix_pages or block_table.shape[1], pages_per_split,
                                total_suffix_pages, sms or groups.sms,
-                               min(MOST_PARTS - pre[1], groups.most_splits))
+                               min(max(1, MOST_PARTS - pre[1]), groups.most_splits))
         done = fast.shared_prefix_attention(
             q, kv_pool, block_table, ctx_len, scale, out, lse_out, groups.packed, pre, tail,
             workspace.parts(groups.batch * groups.q_heads, groups.head_dim, pre[1], tail[1]))
@@ -641,7 +641,7 @@ def shared_prefix_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table:
     pre_pps, pre_splits = groups.splits(total_suffix_pages)
     pps, nsplit = tail_split_plan(B, hq, hkv, max_suffix_pages or max_pages, pages_per_split,
                                   total_suffix_pages, sms or groups.sms,
-                                  min(MOST_PARTS - pre_splits, groups.most_splits))
+                                  min(max(1, MOST_PARTS - pre_splits), groups.most_splits))
     if out is None:
         out = q.new_empty((B, hq, dim))
     else:

@@ -173,3 +173,16 @@ def test_rotary_append_of_one_token_off_a_boundary_to_8_bit_pages(launched, monk
                          on(torch.zeros(1, dtype=torch.int64)))
     assert taken[0].is_contiguous() and taken[0].data_ptr() % 16 == 0
     assert torch.equal(taken[0].as_subclass(torch.Tensor), v.as_subclass(torch.Tensor))
+
+
+@pytest.mark.parametrize("pages", [8 * 1023, 8 * 1024, 8 * 1500, 20_000])
+def test_prefix_in_more_splits_than_the_merge_takes(launched, monkeypatch, pages):
+    """Split sizes of the caller's own that leave no part to the sequences' own pages: the plan
+    ends all the same, and the entry point says what is wrong."""
+    monkeypatch.setattr(paged, "most_splits", lambda *a: 4096)
+    groups = _plan(paged.PrefixGroups, [([0, 1], 16 * pages)], 2, 4, 2, 64, sms=148,
+                   pages_per_split=8)
+    paged.shared_prefix_attention(_bf(2, 4, 64), _bf(8, 2, 2, 16, 64),
+                                  on(torch.zeros((2, pages), dtype=torch.int32)),
+                                  on(torch.zeros(2, dtype=torch.int32)), 0.1, groups)
+    assert launched == ["_shared_prefix"]
